@@ -8,6 +8,8 @@ libagxcuda.so:
     norm       the standalone RMSNorm; rmsnorm_wide_reference
     argmax     the first-maximum rule; argmax_reference
     qmm        the batched tensor-core GEMM (32..256 activation rows)
+    kv4        a paged KV cache held in 4 bits: the append (RoPE and quantisation on the way) and the attention over it
+    sampling   temperature, top-k, top-p and min-p sampling from given random numbers
 
 The reference's numerics module models Apple G17 fp32 arithmetic (flush-to-zero, a software exp2, midpoint-tested
 rsqrt) for its bit-exact references; the B200 kernels use IEEE fp32, so it has no counterpart here.

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "liba
 
 OK, EINVAL, ECUDA, ENCCL, ETIMEOUT, ECORRUPT, ENOMEM, EUNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7
 SCALE_FP16, SCALE_BF16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 TOKEN_UNSET = 0xFFFFFFFF
 EPI_F32, EPI_RES1, EPI_RES2, EPI_SWIGLU = 0, 1, 2, 3
 ROLE_QKV, ROLE_WO, ROLE_GATE, ROLE_UP, ROLE_DOWN, ROLE_HEAD = range(6)
@@ -57,6 +58,34 @@ class EncoderDesc(C.Structure):
                 ("max_batch", C.c_int32), ("max_seq", C.c_int32)]
 
 
+class Kv4Cache(C.Structure):
+    _fields_ = [("data_dev", C.c_void_p), ("pages", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_size", C.c_int32)]
+
+
+class Kv4AppendArgs(C.Structure):
+    _fields_ = [("cache", Kv4Cache), ("qkv_dev", C.c_void_p), ("qkv_ld", C.c_int64), ("qkv_dtype", C.c_int32),
+                ("tokens", C.c_int32), ("heads", C.c_int32), ("positions_dev", C.c_void_p), ("slots_dev", C.c_void_p),
+                ("cos_dev", C.c_void_p), ("sin_dev", C.c_void_p), ("table_rows", C.c_int32), ("bias_dev", C.c_void_p),
+                ("q_norm_dev", C.c_void_p), ("k_norm_dev", C.c_void_p), ("eps", C.c_float), ("qscale", C.c_float),
+                ("q_dev", C.c_void_p), ("q_dtype", C.c_int32)]
+
+
+class Kv4AttentionArgs(C.Structure):
+    _fields_ = [("cache", Kv4Cache), ("q_dev", C.c_void_p), ("out_dev", C.c_void_p), ("dtype", C.c_int32),
+                ("batch", C.c_int32), ("rows", C.c_int32), ("heads", C.c_int32), ("page_table_dev", C.c_void_p),
+                ("table_ld", C.c_int32), ("max_pages", C.c_int32), ("lengths_dev", C.c_void_p),
+                ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [("logits_dev", C.c_void_p), ("logits_ld", C.c_int64), ("dtype", C.c_int32), ("batch", C.c_int32),
+                ("vocab", C.c_int32), ("u_dev", C.c_void_p), ("temperature", C.c_float), ("top_p", C.c_float),
+                ("min_p", C.c_float), ("top_k", C.c_int32), ("temperature_dev", C.c_void_p), ("top_k_dev", C.c_void_p),
+                ("top_p_dev", C.c_void_p), ("min_p_dev", C.c_void_p), ("token_dev", C.c_void_p),
+                ("prob_dev", C.c_void_p)]
+
+
 class Timing(C.Structure):
     _fields_ = [("gpu_ms", C.c_float), ("host_ms", C.c_float), ("launches_per_step", C.c_int32)]
 
@@ -86,6 +115,12 @@ SIGNATURES = {
     "agxc_rope_append_dev": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, C.c_float, _P, _P, _P, _P]),
     "agxc_argmax_dev": (_I, [_P, _P, _I, _P, _P]),
     "agxc_tp_reduce_dev": (_I, [_P, _P, _I, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "agxc_kv4_bytes": (C.c_int64, [C.POINTER(Kv4Cache)]),
+    "agxc_kv4_append_dev": (_I, [_P, C.POINTER(Kv4AppendArgs), _P]),
+    "agxc_kv4_rows_dev": (_I, [_P, C.POINTER(Kv4Cache), _P, _I, _P, _P, _P]),
+    "agxc_kv4_attention_workspace": (C.c_int64, [_P, C.POINTER(Kv4AttentionArgs)]),
+    "agxc_kv4_attention_dev": (_I, [_P, C.POINTER(Kv4AttentionArgs), _P]),
+    "agxc_sample_dev": (_I, [_P, C.POINTER(SampleArgs), _P]),
     "agxc_model_create": (_I, [_P, C.POINTER(ModelDesc), C.POINTER(_P)]),
     "agxc_tp_unique_id": (_I, [_P]),
     "agxc_model_prefill": (_I, [_P, _I, _P, _I, C.POINTER(Timing)]),

@@ -170,6 +170,98 @@ AGXC_API int agxc_tp_reduce_dev(agxc_ctx* ctx, const float* recv_dev, int ranks,
  * the smallest index holding the largest value. (In the decode step this is the vocabulary GEMV's epilogue.) */
 AGXC_API int agxc_argmax_dev(agxc_ctx* ctx, const float* x_dev, int n, int32_t* out_dev, void* stream);
 
+/* ---- a paged KV cache held in 4 bits, its append and its attention, and sampling (no counterpart in the reference,
+ * which keeps one contiguous fp16 cache and chooses greedily) -----------------------------------------------------
+ * The cache: `pages` pages of `page_size` tokens for each of `kv_heads` heads, at data_dev[page][kv_head] as
+ * page_size / 16 tiles of 16 tokens. A tile is K codes (8 head_dim bytes), V codes (8 head_dim bytes) and 16 x
+ * [K, V][group]{scale, bias} fp16: a value is scale * code + bias, per token, KV head and group of 64 dims (the packs'
+ * affine group-64 format). Byte i of a group holds its dims 2i (low nibble) and 2i + 1; with G = head_dim / 64 the
+ * byte of token t, group g is at
+ *     K: t * 32 G + (i / 8) * 8 G + 8 g + i % 8
+ *     V: 8 head_dim + (t / 8) * 256 G + (4 (i / 4) + t % 8 / 2) * 8 G + (t % 2) * 4 G + 4 g + i % 4
+ * (the order in which the attention's lanes read their tensor-core fragments, 16 bytes at a time).
+ * A slot is page * page_size + offset. */
+#define AGXC_F32 0
+#define AGXC_F16 1
+#define AGXC_BF16 2
+typedef struct {
+  void* data_dev;             /* 16-byte aligned */
+  int32_t pages, kv_heads, head_dim, page_size; /* head_dim 64 or 128; page_size a multiple of 16 */
+} agxc_kv4_cache;
+
+/* Bytes of the cache's data (-1: a bad shape). */
+AGXC_API int64_t agxc_kv4_bytes(const agxc_kv4_cache* cache);
+
+typedef struct {
+  agxc_kv4_cache cache;
+  const void* qkv_dev;        /* [tokens][qkv_ld], each [q heads | k heads | v heads] x head_dim */
+  int64_t qkv_ld;
+  int32_t qkv_dtype;          /* AGXC_F32, _F16, _BF16 */
+  int32_t tokens, heads;
+  const int32_t* positions_dev; /* [tokens] rows of the RoPE tables */
+  const int64_t* slots_dev;   /* [tokens] cache places, each at most once; negative: the token is not written */
+  const float* cos_dev;       /* [table_rows][head_dim / 2] */
+  const float* sin_dev;
+  int32_t table_rows;
+  const uint16_t* bias_dev;   /* fp16 [(heads + 2 kv_heads) head_dim] added to the rows first; NULL = none */
+  const uint16_t* q_norm_dev; /* fp16 [head_dim]: RMS norm of each q (k) head before RoPE; both or neither */
+  const uint16_t* k_norm_dev;
+  float eps, qscale;          /* the norm's epsilon; the factor on q after RoPE (log2(e) / sqrt(head_dim)) */
+  void* q_dev;                /* [tokens][heads][head_dim], fp16 or bf16 */
+  int32_t q_dtype;            /* AGXC_F16 or AGXC_BF16 */
+} agxc_kv4_append_args;
+
+/* Rotates each token's q and k (fp32, two rounded products and one rounded sum an output), scales and rounds q, and
+ * writes k and v into the cache in 4 bits. A position outside the tables or a slot past the cache sets the error word
+ * (kErrBadPos) and leaves that token out. tokens = 0 does nothing. */
+AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* args, void* stream);
+
+/* The values the cache holds at `tokens` slots, fp16 [tokens][kv_heads][head_dim] each (zeros for a negative slot). */
+AGXC_API int agxc_kv4_rows_dev(agxc_ctx* ctx, const agxc_kv4_cache* cache, const int64_t* slots_dev, int tokens,
+                               uint16_t* k_dev, uint16_t* v_dev, void* stream);
+
+typedef struct {
+  agxc_kv4_cache cache;
+  const void* q_dev;          /* [batch][rows][heads][head_dim], scaled for the base-2 softmax; fp16 or bf16 */
+  void* out_dev;              /* the same shape and type */
+  int32_t dtype;              /* AGXC_F16 or AGXC_BF16 */
+  int32_t batch, rows, heads;
+  const int32_t* page_table_dev; /* [batch][table_ld]: page of each page_size tokens of a sequence */
+  int32_t table_ld, max_pages;   /* entries a sequence may use: lengths reach at most max_pages * page_size */
+  const int32_t* lengths_dev; /* [batch] tokens held, the rows' own among them */
+  void* workspace_dev;        /* agxc_kv4_attention_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} agxc_kv4_attention_args;
+
+/* Attention over the 4-bit cache for `rows` query rows of each sequence: row i sees keys 0 .. length - rows + i (a row
+ * that sees none gives zeros); q head h reads KV head h / (heads / kv_heads). A length outside 0 .. max_pages *
+ * page_size is clamped and a page outside the cache is read as no keys; both set the error word (kErrBadPos). */
+AGXC_API int64_t agxc_kv4_attention_workspace(agxc_ctx* ctx, const agxc_kv4_attention_args* args);
+AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args* args, void* stream);
+
+typedef struct {
+  const void* logits_dev;     /* [batch][logits_ld] */
+  int64_t logits_ld;
+  int32_t dtype;              /* AGXC_F32, _F16, _BF16 */
+  int32_t batch, vocab;
+  const float* u_dev;         /* [batch] uniform numbers in [0, 1) */
+  float temperature, top_p, min_p; /* used where the array below is NULL */
+  int32_t top_k;
+  const float* temperature_dev; /* [batch], each nullable */
+  const int32_t* top_k_dev;
+  const float* top_p_dev;
+  const float* min_p_dev;
+  int32_t* token_dev;         /* [batch] */
+  float* prob_dev;            /* [batch], nullable */
+} agxc_sample_args;
+
+/* One token a row. Tokens are ranked by logit, equal logits by index (NaN ranks as -inf). Weights are exp((l - max) / T)
+ * in whole units of 2^-40, so every sum is exact and no result depends on an order of addition. Kept: the first top_k
+ * ranks (top_k <= 0: all); of those the ranks whose weight before them is below ceil(top_p * total) (top_p >= 1: all,
+ * and always the first); of those the weights >= min_p. The token is the first kept index whose cumulative weight
+ * exceeds floor(u * total), and prob its weight / total. T = 0: the first maximum, prob 1. No finite logit: -1, 0. */
+AGXC_API int agxc_sample_dev(agxc_ctx* ctx, const agxc_sample_args* args, void* stream);
+
 /* ---- the model (agxforge/inference/assemble.py configure 71-92, build 596-828; models.py 26-54) -------------- */
 typedef struct {
   int32_t d_model, n_layers, n_heads, n_kv_heads, head_dim, ffn, vocab;
