@@ -1,8 +1,28 @@
 // kv4_attention.cu — attention over the paged 4-bit KV cache (kv4.cuh): query row i of a sequence of length L with n
-// rows sees keys 0 .. L - n + i, out = sum_t p_t v_t / sum_t p_t with p_t = 2^(q . k_t - m), one pass over the keys with
-// a running maximum; k and v are scale * code + bias per group of 64 dims.
+// rows sees keys 0 .. L - n + i, out = sum_t p_t v_t / sum_t p_t with p_t = 2^(q . k_t - m), one pass over the keys.
 //
-// One CTA of 4 warps per (sequence, row, head), a warp a key at a time.
+// Mathematics. With k = s code + b per group of 64 dims, q . k = sum_g s_g (q_g . code_g) + b_g sum(q_g), and
+// sum_t p_t v_t = sum_t (p_t s_t) code_t + sum_t p_t b_t: the codes meet the tensor cores as they are (a 4-bit field
+// masked out of a word IS an fp16 subnormal, code 2^-24 or code 2^-20, so one AND prepares two operands), and scales
+// and biases are applied to the 16 x 8 scores, not to the 16 x head_dim values. A warp takes 32 keys at a time, as two
+// tiles of 16:
+//   scores   D[key][column] = codes (A, 16 keys x 16 dims) x q (B, 16 dims x 8 columns), a column = one (row, head)
+//   values   O[dim][column] += (codes - 8) (A, 16 dims x 16 keys) x P (B, 16 keys x 8 columns); the score fragments
+//            become P operands by one 8 x 8 transpose each (movmatrix)
+// q is scaled by a power of two a column and the fields' 2^-24 is undone in fp32 (exact). P = p s / sref is rounded to
+// fp16 (11 bits; the only rounding of the pass): sref is the running power of two above the group's scales and the
+// reference m sits 8 below the running maximum, so P stays in fp16's normal range down to 2^-22 of the largest weight.
+// The values' codes are taken about 8 (fields or-ed into 1024 + code, minus 1032: exact) and their bias as b + 8 s, so
+// that P's rounding counts by a value's distance from its group's middle and the sums over thousands of keys stay
+// small beside what the tensor core's accumulation drops (codes of one sign: 3.6e-4 off at 8,192 keys, 2-norm; about 8:
+// 2.8e-4, of which the output's own fp16 rounding is 2.1e-4). m and sref move only when a score passes m + 12 or a
+// scale passes 8 sref (one vote for 32 keys), which rescales the accumulators.
+//
+// Split. The 32-key units of every (sequence, KV head, block of columns) lie end to end; each CTA takes an equal share
+// of that line, whatever the lengths are, and its four warps take its units in turn. A piece that is not a whole item
+// leaves its maximum, sum and values in the workspace, and a second kernel joins the pieces in a fixed order (no
+// atomics: equal calls give equal bits). A warp has two units of shared memory and copies one (a bulk copy a tile, which
+// is contiguous) while it computes on the other.
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -10,81 +30,675 @@
 namespace agxc {
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kNone = -1e30f;         // the maximum that stands for no key
+
 struct Kv4AttnParams {
   Kv4 c;
   const void* q;
   void* out;
-  int bf16, B, n, H, table_ld, max_pages;
+  int B, n, H, G, CB;                   // G = q heads a KV head, CB = column blocks an item row
+  int table_ld, max_pages, ctas;
   const int32_t* table;
   const int32_t* lengths;
+  float* part;                          // [2 ctas][columns]{max, sum}, then [2 ctas][columns][hd]
   unsigned* err;
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-template <int HD, typename T>
-__global__ void __launch_bounds__(128) kv4_attn_simple(const __grid_constant__ Kv4AttnParams p) {
-  using Tile = Kv4Tile<HD>;
-  constexpr int E = HD / 32;
-  const int h = blockIdx.x % p.H, i = blockIdx.x / p.H % p.n, b = blockIdx.x / p.H / p.n;
-  const int j = h / (p.H / p.c.kvh), warp = threadIdx.x >> 5, l = threadIdx.x & 31;
-  int len = p.lengths[b];
-  const int64_t most = static_cast<int64_t>(p.max_pages) * p.c.page;
+__device__ __forceinline__ int seq_len(const Kv4AttnParams& p, int b) {
+  const int len = p.lengths[b];
+  const int most = p.max_pages * p.c.page;
   if (len < 0 || len > most) {
-    if (threadIdx.x == 0) atomicOr(p.err, kErrBadPos);
-    len = len < 0 ? 0 : static_cast<int>(most);
+    atomicOr(p.err, kErrBadPos);
+    return len < 0 ? 0 : most;
   }
-  const int keys = len - p.n + i + 1;
-  const int64_t row = (static_cast<int64_t>(b) * p.n + i) * p.H + h;
-  float q[E], o[E] = {}, m = -FLT_MAX, sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = to_f(static_cast<const T*>(p.q)[row * HD + l * E + e]);
-  const int g = l * E / 64, byte = l * E % 64 / 2;
-  for (int t = warp; t < keys; t += 4) {
-    const int page = p.table[static_cast<int64_t>(b) * p.table_ld + t / p.c.page], tt = t & 15;
-    if (page < 0 || page >= p.c.pages) {
-      if (l == 0) atomicOr(p.err, kErrBadPos);
-      continue;
-    }
-    const uint8_t* tile = Tile::ptr(p.c, page, j, t % p.c.page >> 4);
-    const __half2* sb = reinterpret_cast<const __half2*>(tile + Tile::kSb + tt * Tile::kEntry);
-    const float2 ks = __half22float2(sb[g]), vs = __half22float2(sb[Tile::G + g]);
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const unsigned c = tile[Tile::k_at(tt, g, byte + e / 2)] >> (4 * (e & 1)) & 15;
-      s += q[e] * (static_cast<float>(c) * ks.x + ks.y);
-    }
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), f = exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    sum = sum * f + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const unsigned c = tile[Tile::v_at(tt, g, byte + e / 2)] >> (4 * (e & 1)) & 15;
-      o[e] = o[e] * f + w * (static_cast<float>(c) * vs.x + vs.y);
+  return len;
+}
+
+__device__ __forceinline__ int units_of(int len) { return (len + 31) >> 5; }
+
+// A CTA's place on the line of units: sequence b, item = kv_head * CB + column block, unit t of its T, and how many
+// units are left of the CTA's share.
+struct Place {
+  int b, item, t, T, len;
+  long long rem;
+  __device__ int end() const { return rem < T - t ? t + static_cast<int>(rem) : T; }
+  __device__ void next(const Kv4AttnParams& p) {
+    rem -= end() - t;
+    t = 0;
+    if (++item == p.c.kvh * p.CB) {
+      item = 0;
+      do {
+        if (++b >= p.B) {
+          rem = 0;
+          return;
+        }
+        len = seq_len(p, b);
+        T = units_of(len);
+      } while (T == 0);
     }
   }
-  __shared__ float so[4][HD], sm[4], ss[4];
+};
+
+// Units a CTA: the line's length over the CTAs, a multiple of the warps. Every warp computes it for itself.
+__device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < p.B; b += 32) sum += units_of(seq_len(p, b));
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][l * E + e] = o[e];
-  if (l == 0) {
-    sm[warp] = m;
-    ss[warp] = sum;
+  for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  sum *= p.c.kvh * p.CB;
+  const long long per = (sum + p.ctas - 1) / p.ctas;
+  return (per + kWarps - 1) / kWarps * kWarps;
+}
+
+// The sequence that holds position `at` of the line, and where its items start.
+__device__ __forceinline__ bool line_find(const Kv4AttnParams& p, int lane, long long at, int& seq, int& len,
+                                          long long& start) {
+  long long acc = 0;
+  const int items = p.c.kvh * p.CB;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    const int l = b < p.B ? seq_len(p, b) : 0;
+    const long long mine = static_cast<long long>(units_of(l)) * items;
+    long long up = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, up, m);
+      if (lane >= m) up += o;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, acc + up > at);
+    if (past) {
+      const int w = __ffs(past) - 1;
+      seq = b0 + w;
+      len = __shfl_sync(0xffffffffu, l, w);
+      start = acc + __shfl_sync(0xffffffffu, up - mine, w);
+      return true;
+    }
+    acc += __shfl_sync(0xffffffffu, up, 31);
   }
-  __syncthreads();
-  const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float den = 0.f;
-  for (int w = 0; w < 4; ++w) den += ss[w] * exp2f(sm[w] - mm);
-  for (int d = threadIdx.x; d < HD; d += 128) {
-    float v = 0.f;
-    for (int w = 0; w < 4; ++w) v += so[w][d] * exp2f(sm[w] - mm);
-    static_cast<T*>(p.out)[row * HD + d] = static_cast<T>(den > 0.f ? v / den : 0.f);
+  return false;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
+
+// code - 8 of the even (hi = 0) or 16 (code - 8) of the odd nibble in the low byte of each half of x, in fp16 (exact)
+__device__ __forceinline__ uint32_t about8(uint32_t x, int hi) {
+  const uint32_t u = (x & (hi ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + code, or 1024 + 16 code
+  const __half2 d = __hsub2(as_half2(u), as_half2(hi ? 0x64806480u : 0x64086408u));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// D = A B, m16n8k16
+__device__ __forceinline__ void mma_16816_zero(float& d0, float& d1, float& d2, float& d3, uint32_t a0, uint32_t a1,
+                                               uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};\n"
+      : "=f"(d0), "=f"(d1), "=f"(d2), "=f"(d3)
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ void unpack8(const uint4& u, float* f, const __half*) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = bits_float2(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+__device__ __forceinline__ void unpack8(const uint4& u, float* f, const __nv_bfloat16*) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* f);
+template <>
+__device__ __forceinline__ uint4 pack8<__half>(const float* f) {
+  return make_uint4(half2_bits(f[0], f[1]), half2_bits(f[2], f[3]), half2_bits(f[4], f[5]), half2_bits(f[6], f[7]));
+}
+template <>
+__device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Shared memory of a CTA: rings [warp][stage] of units, the warps' results [warp][column][hd + 4], {max, sum} of each,
+// barriers and the tiles that were copied [warp][stage].
+template <int HD, int NT>
+struct Smem {
+  static constexpr int kStages = NT == 1 ? 2 : 3;
+  static constexpr int kStage = 2 * Kv4Tile<HD>::kBytes;
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kRow = HD + 4;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kO = kRing;
+  static constexpr int kMl = kO + kWarps * kCols * kRow * 4;
+  static constexpr int kBar = kMl + kWarps * kCols * 8;
+  static constexpr int kCame = kBar + kWarps * kStages * 8;
+  static constexpr int kBytes = kCame + kWarps * kStages * 4;
+};
+
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+  using Tile = Kv4Tile<HD>;
+  using Sm = Smem<HD, NT>;
+  constexpr int GR = HD / 64;               // groups of 64 dims
+  constexpr int S = Sm::kStages, NC = Sm::kCols;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  uint8_t* ring = sm + warp * S * Sm::kStage;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Sm::kBar) + warp * S;
+  volatile unsigned* came = reinterpret_cast<unsigned*>(sm + Sm::kCame) + warp * S;
+  float* so = reinterpret_cast<float*>(sm + Sm::kO);
+  float2* sml = reinterpret_cast<float2*>(sm + Sm::kMl);
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&bar[i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const long long quota = line_quota(p, lane);
+  Place at;
+  {
+    const long long from = quota * blockIdx.x;
+    long long start;
+    if (quota == 0 || !line_find(p, lane, from, at.b, at.len, start)) return;  // every warp of the CTA alike
+    at.T = units_of(at.len);
+    const long long off = from - start;
+    at.item = static_cast<int>(off / at.T);
+    at.t = static_cast<int>(off % at.T);
+    at.rem = quota;
+  }
+  const int tiles_page = p.c.page >> 4;
+  // where the units end that some column of the item's block sees
+  auto seen = [&](const Place& w) {
+    const int last = min(p.n - 1, (w.item % p.CB * NC + NC - 1) / p.G);
+    const int keys = w.len - p.n + last + 1;
+    return keys > 0 ? min(w.end(), units_of(keys)) : 0;
+  };
+
+  // The warp's copies run S units ahead of its reads; `ahead` walks the line on its own. Lanes 0 and 1 look after the
+  // unit's first and second tile: the page (fetched a unit early) and the tile's place in it.
+  Place ahead = at;
+  int a_unit, a_end, a_slot = 0, flying = 0, a_page = -1, a_in = 0, a_idx = 0, a_tiles = 0;
+  const int32_t* a_row = nullptr;
+  const uint8_t* a_head = nullptr;
+  bool dead = false, more = true;
+  auto enter = [&]() {  // the warp's first unit of the place `ahead` has come to
+    a_unit = ahead.t + warp;
+    a_end = seen(ahead);
+    const int tile = 2 * a_unit + (lane & 1);
+    a_idx = tile / tiles_page;
+    a_in = tile % tiles_page;
+    a_tiles = (ahead.len + 15) >> 4;
+    a_row = p.table + static_cast<long long>(ahead.b) * p.table_ld;
+    a_head = p.c.data + static_cast<size_t>(ahead.item / p.CB) * tiles_page * Tile::kBytes;
+  };
+  auto settle = [&]() {  // the next unit that exists, and its pages
+    while (a_unit >= a_end) {
+      ahead.next(p);
+      if (ahead.rem <= 0) {
+        more = false;
+        return;
+      }
+      enter();
+    }
+    if (lane < 2 && 2 * a_unit + lane < a_tiles) a_page = __ldg(a_row + a_idx);
+  };
+  const size_t page_bytes = static_cast<size_t>(p.c.kvh) * tiles_page * Tile::kBytes;
+  auto issue = [&]() {
+    if (!more || dead) return;
+    const bool mine = lane < 2 && 2 * a_unit + lane < a_tiles;
+    const bool ok = mine && static_cast<unsigned>(a_page) < static_cast<unsigned>(p.c.pages);
+    if (mine && !ok) atomicOr(p.err, kErrBadPos);
+    const unsigned mask = __ballot_sync(0xffffffffu, ok);
+    if (lane == 0) {
+      came[a_slot] = mask;
+      mbar_arrive_expect_tx(&bar[a_slot], __popc(mask) * Tile::kBytes);
+    }
+    __syncwarp();
+    if (ok)
+      bulk_g2s(ring + a_slot * Sm::kStage + lane * Tile::kBytes, a_head + a_page * page_bytes + a_in * Tile::kBytes,
+               Tile::kBytes, &bar[a_slot]);
+    a_slot = a_slot + 1 == S ? 0 : a_slot + 1;
+    ++flying;
+    a_unit += kWarps;
+    a_in += 2 * kWarps;
+    while (a_in >= tiles_page) {
+      a_in -= tiles_page;
+      ++a_idx;
+    }
+    settle();
+  };
+  enter();
+  settle();
+  for (int i = 0; i < S; ++i) issue();
+
+  int slot = 0, phase = 0;
+  while (at.rem > 0) {
+    const int j = at.item / p.CB, col0 = at.item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
+    // q as B fragments: word w of a lane's 8 or 16 bytes of codes holds dims 8w .. 8w + 7 of its chunk, and its four
+    // masks give dims (0, 4), (1, 5) 2^4, (2, 6), (3, 7) 2^4
+    uint32_t qf[NT][GR][2][4];
+    float unq[NT][2], qsum[NT][GR][2];      // of columns 2c, 2c + 1: 2^24 over q's factor, and sum(q_g) / unq
+    int lim[NT][2];                         // keys a column sees
+    int least = 0x7fffffff, most = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + r;
+      float f[GR][16], mx = 0.f;
+      const bool live = col < cols;
+      const int i = (col0 + col) / p.G;
+      const T* src = static_cast<const T*>(p.q) +
+                     ((static_cast<long long>(at.b) * p.n + i) * p.H + j * p.G + (col0 + col) % p.G) * HD + 16 * c;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        const uint4 u0 = live ? *reinterpret_cast<const uint4*>(src + 64 * g) : make_uint4(0, 0, 0, 0);
+        const uint4 u1 = live ? *reinterpret_cast<const uint4*>(src + 64 * g + 8) : make_uint4(0, 0, 0, 0);
+        unpack8(u0, f[g], static_cast<const T*>(nullptr));
+        unpack8(u1, f[g] + 8, static_cast<const T*>(nullptr));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(f[g][e]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^x with x = 8 - floor(log2 max): the largest |q| becomes 2^8 .. 2^9
+      const int ex = mx > 1e-35f ? static_cast<int>(__float_as_uint(mx) >> 23) : 127;
+      const float up = __uint_as_float(static_cast<uint32_t>(min(max(262 - ex, 30), 230)) << 23);
+      const float down = 16777216.f / up;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += f[g][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum /= down;
+        qsum[nt][g][0] = __shfl_sync(0xffffffffu, sum, 8 * c);
+        qsum[nt][g][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const float* h = f[g] + 8 * w;
+          qf[nt][g][w][0] = half2_bits(h[0] * up, h[4] * up);
+          qf[nt][g][w][1] = half2_bits(h[1] * up * 0.0625f, h[5] * up * 0.0625f);
+          qf[nt][g][w][2] = half2_bits(h[2] * up, h[6] * up);
+          qf[nt][g][w][3] = half2_bits(h[3] * up * 0.0625f, h[7] * up * 0.0625f);
+        }
+      }
+      unq[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);
+      unq[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int cc = nt * 8 + 2 * c + e;
+        lim[nt][e] = cc < cols ? max(0, at.len - p.n + (col0 + cc) / p.G + 1) : 0;
+      }
+    }
+    // keys that every (any) column of the block sees
+    least = max(0, at.len - p.n + col0 / p.G + 1);
+    most = max(0, at.len - p.n + (col0 + cols - 1) / p.G + 1);
+
+    float o[NT][GR][4][4], m[NT][2], l[NT][2], bt[NT][GR][2], sref[GR], isref[GR], big[GR];
+#pragma unroll
+    for (int g = 0; g < GR; ++g) sref[g] = 5.9604645e-8f, isref[g] = 16777216.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = 0.f;
+        l[nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        bt[nt][g][0] = bt[nt][g][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[nt][g][k][0] = o[nt][g][k][1] = o[nt][g][k][2] = o[nt][g][k][3] = 0.f;
+      }
+    }
+
+    const int end = seen(at);
+    bool fresh = true;                       // no key yet: m is set, up or down, by the first unit
+    for (int unit = at.t + warp; unit < end; unit += kWarps) {
+      if (!dead && !mbar_wait_bounded(&bar[slot], phase, p.err)) dead = true;
+      if (dead) continue;
+      --flying;
+      const unsigned mask = came[slot];
+      const uint8_t* st = ring + slot * Sm::kStage;
+      float y[2][NT][4];                     // log2 of the weights of (key r, columns 2c, 2c + 1), (key r + 8, the same)
+      uint32_t ve[2][2][GR];                 // V's {scale, bias} of keys r, r + 8
+      bool move = fresh;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* tl = st + h * Tile::kBytes;
+        // K words and entries of keys r and r + 8
+        uint32_t kw[2][2 * GR], ke[2][GR];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (GR == 2) {
+            const uint4 k4 = *reinterpret_cast<const uint4*>(tl + i * 512 + lane * 16);
+            kw[i][0] = k4.x; kw[i][1] = k4.y; kw[i][2] = k4.z; kw[i][3] = k4.w;
+            const uint4 e4 = *reinterpret_cast<const uint4*>(tl + Tile::kSb + (r + 8 * i) * 16);
+            ke[i][0] = e4.x; ke[i][1] = e4.y; ve[h][i][0] = e4.z; ve[h][i][1] = e4.w;
+          } else {
+            const uint2 k2 = *reinterpret_cast<const uint2*>(tl + i * 256 + lane * 8);
+            kw[i][0] = k2.x; kw[i][1] = k2.y;
+            const uint2 e2 = *reinterpret_cast<const uint2*>(tl + Tile::kSb + (r + 8 * i) * 8);
+            ke[i][0] = e2.x; ve[h][i][0] = e2.y;
+          }
+        }
+        float d[NT][GR][4];
+#pragma unroll
+        for (int g = 0; g < GR; ++g)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t a = kw[0][2 * g + w], b = kw[1][2 * g + w], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t f0 = a & 0x000f000fu, f1 = b & 0x000f000fu, f2 = a & 0x00f000f0u, f3 = b & 0x00f000f0u;
+            const uint32_t e0 = a8 & 0x000f000fu, e1 = b8 & 0x000f000fu, e2 = a8 & 0x00f000f0u, e3 = b8 & 0x00f000f0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float* x = d[nt][g];
+              if (w == 0) mma_16816_zero(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][0], qf[nt][g][w][1]);
+              else mma_16816(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][0], qf[nt][g][w][1]);
+              mma_16816(x[0], x[1], x[2], x[3], e0, e1, e2, e3, qf[nt][g][w][2], qf[nt][g][w][3]);
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float2 sb[GR];
+#pragma unroll
+          for (int g = 0; g < GR; ++g) sb[g] = bits_float2(ke[i][g]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = sb[0].y * qsum[nt][0][e];
+              if (GR == 2) v = fmaf(sb[GR - 1].y, qsum[nt][GR - 1][e], v);
+#pragma unroll
+              for (int g = 0; g < GR; ++g) v = fmaf(sb[g].x, d[nt][g][2 * i + e], v);
+              y[h][nt][2 * i + e] = fmaf(v, unq[nt][e], -m[nt][e]);
+            }
+        }
+      }
+      if (unit * 32 + 32 > least || mask != 3u) {  // the mask's edge: an unseen key weighs nothing, whatever its bytes hold
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = mask >> h & 1 ? unit * 32 + h * 16 + r + 8 * i : 0x7fffffff;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (key >= lim[nt][e]) y[h][nt][2 * i + e] = -INFINITY;
+            if (key >= most) {
+#pragma unroll
+              for (int g = 0; g < GR; ++g) ve[h][i][g] = 0u;
+            }
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        move |= fmaxf(fmaxf(fmaxf(y[0][nt][0], y[0][nt][1]), fmaxf(y[0][nt][2], y[0][nt][3])),
+                      fmaxf(fmaxf(y[1][nt][0], y[1][nt][1]), fmaxf(y[1][nt][2], y[1][nt][3]))) > 12.f;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {  // the low halves of the entries: V's scales
+        const __half2 a = __hmax2(__habs2(as_half2(ve[0][0][g])), __habs2(as_half2(ve[0][1][g])));
+        const __half2 b = __hmax2(__habs2(as_half2(ve[1][0][g])), __habs2(as_half2(ve[1][1][g])));
+        big[g] = __low2float(__hmax2(a, b));
+        move |= big[g] > 8.f * sref[g];
+      }
+      if (mask != 0u && __any_sync(0xffffffffu, move)) {
+        float fg[GR];
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          const float up = fmaxf(sref[g], __uint_as_float((__float_as_uint(warp_max(big[g])) + 0x7fffffu) & 0x7f800000u));
+          fg[g] = sref[g] / up;
+          sref[g] = up;
+          isref[g] = 1.f / up;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(y[0][nt][e], y[0][nt][2 + e]), fmaxf(y[1][nt][e], y[1][nt][2 + e]));
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            // the reference goes up by this much; a column that sees none of the first unit's keys sees no later ones
+            const float by = fresh ? (mx > -INFINITY ? mx - 8.f : 0.f) : fmaxf(0.f, mx - 8.f);
+            const float f = fresh ? 1.f : ex2(-by);
+            m[nt][e] += by;
+            l[nt][e] *= f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              y[h][nt][e] -= by;
+              y[h][nt][2 + e] -= by;
+            }
+#pragma unroll
+            for (int g = 0; g < GR; ++g) {
+              bt[nt][g][e] *= f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                o[nt][g][k][e] *= f * fg[g];
+                o[nt][g][k][2 + e] *= f * fg[g];
+              }
+            }
+          }
+      }
+      if (mask != 0u) fresh = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // weights: P operands, the sum, and the bias term
+        uint32_t pf[NT][GR][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float s1[GR], b8[GR];
+#pragma unroll
+          for (int g = 0; g < GR; ++g) {
+            const float2 e2 = bits_float2(ve[h][i][g]);
+            s1[g] = e2.x * isref[g];
+            b8[g] = fmaf(8.f, e2.x, e2.y);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float p0 = ex2(y[h][nt][2 * i]), p1 = ex2(y[h][nt][2 * i + 1]);
+            l[nt][0] += p0;
+            l[nt][1] += p1;
+#pragma unroll
+            for (int g = 0; g < GR; ++g) {
+              bt[nt][g][0] = fmaf(p0, b8[g], bt[nt][g][0]);
+              bt[nt][g][1] = fmaf(p1, b8[g], bt[nt][g][1]);
+              pf[nt][g][i] = transpose8(half2_bits(p0 * s1[g], p1 * s1[g]));
+            }
+          }
+        }
+        // values of keys 2c, 2c + 1, 2c + 8, 2c + 9: rows r hold the even nibbles, rows r + 8 the odd ones (2^4 larger)
+        const uint8_t* tl = st + h * Tile::kBytes + Tile::kCodes;
+        uint32_t vw[4][GR];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (GR == 2) {
+            const uint4 v4 = *reinterpret_cast<const uint4*>(tl + i * 512 + lane * 16);
+            vw[2 * i][0] = v4.x; vw[2 * i][1] = v4.y; vw[2 * i + 1][0] = v4.z; vw[2 * i + 1][1] = v4.w;
+          } else {
+            const uint2 v2 = *reinterpret_cast<const uint2*>(tl + i * 256 + lane * 8);
+            vw[2 * i][0] = v2.x; vw[2 * i + 1][0] = v2.y;
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          const uint32_t xa = prmt(vw[0][g], vw[1][g], 0x5410u), xb = prmt(vw[2][g], vw[3][g], 0x5410u);
+          const uint32_t ya = prmt(vw[0][g], vw[1][g], 0x7632u), yb = prmt(vw[2][g], vw[3][g], 0x7632u);
+          const uint32_t a[4] = {xa, xa >> 8, ya, ya >> 8}, b[4] = {xb, xb >> 8, yb, yb >> 8};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a0 = about8(a[k], 0), a1 = about8(a[k], 1), a2 = about8(b[k], 0), a3 = about8(b[k], 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816(o[nt][g][k][0], o[nt][g][k][1], o[nt][g][k][2], o[nt][g][k][3], a0, a1, a2, a3, pf[nt][g][0],
+                        pf[nt][g][1]);
+          }
+        }
+      }
+      __syncwarp();                        // every lane has read the unit: the next copy may overwrite it
+      issue();
+      slot = slot + 1 == S ? 0 : slot + 1;
+      if (slot == 0) phase ^= 1;
+    }
+
+    // the warp's result: a lane holds dims 64 g + 8 r + (0 .. 7) of columns 2c, 2c + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = nt * 8 + 2 * c + e;
+        float sum = l[nt][e];
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (r == 0) sml[warp * NC + col] = make_float2(sum > 0.f ? m[nt][e] : kNone, sum);
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          float bias = bt[nt][g][e];
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) bias += __shfl_xor_sync(0xffffffffu, bias, x);
+          const float f0 = sref[g], f1 = 0.0625f * sref[g];
+          float* dst = so + (warp * NC + col) * Sm::kRow + 64 * g + 8 * r;
+          *reinterpret_cast<float4*>(dst) =
+              make_float4(fmaf(o[nt][g][0][e], f0, bias), fmaf(o[nt][g][0][2 + e], f1, bias),
+                          fmaf(o[nt][g][1][e], f0, bias), fmaf(o[nt][g][1][2 + e], f1, bias));
+          *reinterpret_cast<float4*>(dst + 4) =
+              make_float4(fmaf(o[nt][g][2][e], f0, bias), fmaf(o[nt][g][2][2 + e], f1, bias),
+                          fmaf(o[nt][g][3][e], f0, bias), fmaf(o[nt][g][3][2 + e], f1, bias));
+        }
+      }
+    __syncthreads();
+    // the four warps joined; whole items are written out, pieces go to the workspace
+    const bool whole = at.t == 0 && at.end() == at.T;
+    const int piece = 2 * blockIdx.x + (at.t == 0 ? 1 : 0);
+    for (int u = threadIdx.x; u < cols * (HD / 8); u += kThreads) {
+      const int col = u / (HD / 8), d = u % (HD / 8) * 8;
+      float2 ml[kWarps];
+      float mx = kNone, sum = 0.f, v[8] = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        ml[w] = sml[w * NC + col];
+        mx = fmaxf(mx, ml[w].x);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(ml[w].x - mx);
+        sum += f * ml[w].y;
+        const float* src = so + (w * NC + col) * Sm::kRow + d;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(f, src[e], v[e]);
+      }
+      if (whole) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        const int i = (col0 + col) / p.G;
+        T* dst = static_cast<T*>(p.out) +
+                 ((static_cast<long long>(at.b) * p.n + i) * p.H + j * p.G + (col0 + col) % p.G) * HD + d;
+        *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
+      } else {
+        float* ml_out = p.part + (static_cast<long long>(piece) * NC + col) * 2;
+        float* dst = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2 + (static_cast<long long>(piece) * NC + col) * HD + d;
+        if (d == 0) *reinterpret_cast<float2*>(ml_out) = make_float2(mx, sum);
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+    __syncthreads();
+    at.next(p);
+  }
+  // a wait that gave up left copies in flight: they land before the CTA's memory is another's
+  if (dead)
+    for (int i = 0; i < flying; ++i) {
+      mbar_wait_bounded(&bar[slot], phase, p.err);
+      slot = slot + 1 == S ? 0 : slot + 1;
+      if (slot == 0) phase ^= 1;
+    }
+}
+
+// One CTA an item: joins the pieces that the CTAs of kv4_attn_kernel left of it, in their order; writes zeros for a
+// sequence of no tokens.
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int NC = 8 * NT;
+  const int lane = threadIdx.x & 31;
+  const int items = p.c.kvh * p.CB, b = blockIdx.x / items, item = blockIdx.x % items;
+  pdl_wait();
+  const int units = units_of(seq_len(p, b));
+  const int j = item / p.CB, col0 = item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
+  long long c0 = 0, c1 = 0;
+  if (units) {
+    const long long quota = line_quota(p, lane);
+    long long before = 0;
+    for (int x = lane; x < b; x += 32) before += units_of(seq_len(p, x));
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) before += __shfl_xor_sync(0xffffffffu, before, m);
+    const long long start = before * items + static_cast<long long>(item) * units;
+    c0 = start / quota;
+    c1 = (start + units - 1) / quota;
+    if (c0 == c1) return;                   // one CTA had all of it
+  }
+  for (int u = threadIdx.x; u < cols * (HD / 8); u += kThreads) {
+    const int col = u / (HD / 8), d = u % (HD / 8) * 8;
+    float v[8] = {};
+    if (units) {
+      const float* ml = p.part;
+      const float* val = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2;
+      float mx = kNone, sum = 0.f;
+      for (long long x = c0; x <= c1; ++x)
+        mx = fmaxf(mx, __ldcg(ml + ((2 * x + (x == c0)) * NC + col) * 2));
+      for (long long x = c0; x <= c1; ++x) {
+        const long long k = (2 * x + (x == c0)) * NC + col;
+        const float2 q = __ldcg(reinterpret_cast<const float2*>(ml) + k);
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d));
+        const float4 e = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d + 4));
+        const float f = ex2(q.x - mx);
+        sum = fmaf(f, q.y, sum);
+        v[0] = fmaf(f, a.x, v[0]); v[1] = fmaf(f, a.y, v[1]); v[2] = fmaf(f, a.z, v[2]); v[3] = fmaf(f, a.w, v[3]);
+        v[4] = fmaf(f, e.x, v[4]); v[5] = fmaf(f, e.y, v[5]); v[6] = fmaf(f, e.z, v[6]); v[7] = fmaf(f, e.w, v[7]);
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= inv;
+    }
+    const int i = (col0 + col) / p.G;
+    T* dst = static_cast<T*>(p.out) +
+             ((static_cast<long long>(b) * p.n + i) * p.H + j * p.G + (col0 + col) % p.G) * HD + d;
+    *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
   }
 }
 
@@ -104,6 +718,46 @@ int attn_check(const agxc_kv4_attention_args* a) {
   return 0;
 }
 
+// The launch's shape: 16 columns a block where one row's heads do not fill 8, and as many CTAs as the GPU holds at once
+// (four an SM with 8 columns, two with 16), or fewer where the longest lengths possible make fewer than four units each.
+struct Shape {
+  int nt, cb, ctas;
+  int64_t bytes(int hd) const { return static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
+};
+
+Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
+  Shape s;
+  const int64_t cols = static_cast<int64_t>(a->rows) * (a->heads / a->cache.kv_heads);
+  s.nt = cols > 8 ? 2 : 1;
+  s.cb = static_cast<int>((cols + 8 * s.nt - 1) / (8 * s.nt));
+  const int64_t units = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb *
+                        ((static_cast<int64_t>(a->max_pages) * a->cache.page_size + 31) / 32);
+  const int64_t full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 4 : 2);
+  const int64_t want = (units + kWarps - 1) / kWarps;
+  s.ctas = static_cast<int>(want < 1 ? 1 : want < full ? want : full);
+  return s;
+}
+
+template <int HD, int NT, typename T>
+int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
+  constexpr int smem = Smem<HD, NT>::kBytes;
+  static bool allowed[64] = {};
+  int dev = 0;
+  AGXC_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && !allowed[dev]) {
+    AGXC_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    allowed[dev] = true;
+  }
+  if (int rc = launch_ex(kv4_attn_kernel<HD, NT, T>, dim3(p.ctas), dim3(kThreads), smem, s, 1, p)) return rc;
+  return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(kThreads), 0, s,
+                   1, p);
+}
+
+template <int HD, typename T>
+int attn_launch_nt(const Kv4AttnParams& p, int nt, cudaStream_t s) {
+  return nt == 1 ? attn_launch<HD, 1, T>(p, s) : attn_launch<HD, 2, T>(p, s);
+}
+
 }  // namespace
 }  // namespace agxc
 
@@ -114,7 +768,7 @@ extern "C" {
 AGXC_API int64_t agxc_kv4_attention_workspace(agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   if (!ctx) return fail(AGXC_EINVAL, "kv4_attention: null context");
   if (attn_check(a)) return -1;
-  return 0;
+  return attn_shape(ctx, a).bytes(a->cache.head_dim);
 }
 
 AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args* a, void* stream) {
@@ -125,22 +779,21 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
     return fail(AGXC_EINVAL, "kv4_attention: null buffer");
   if (reinterpret_cast<uintptr_t>(a->q_dev) % 16 || reinterpret_cast<uintptr_t>(a->out_dev) % 16)
     return fail(AGXC_EINVAL, "kv4_attention: q and out must be 16-byte aligned");
+  const Shape sh = attn_shape(ctx, a);
+  if (a->workspace_bytes < sh.bytes(a->cache.head_dim) || !a->workspace_dev ||
+      reinterpret_cast<uintptr_t>(a->workspace_dev) % 16)
+    return fail(AGXC_EINVAL, "kv4_attention: a 16-byte aligned workspace of agxc_kv4_attention_workspace bytes");
   Kv4AttnParams p;
   p.c = kv4_of(a->cache);
-  p.q = a->q_dev; p.out = a->out_dev; p.bf16 = a->dtype == AGXC_BF16; p.B = a->batch; p.n = a->rows; p.H = a->heads;
+  p.q = a->q_dev; p.out = a->out_dev; p.B = a->batch; p.n = a->rows; p.H = a->heads;
+  p.G = a->heads / a->cache.kv_heads; p.CB = sh.cb; p.ctas = sh.ctas;
   p.table_ld = a->table_ld; p.max_pages = a->max_pages; p.table = a->page_table_dev; p.lengths = a->lengths_dev;
-  p.err = ctx->err_dev;
+  p.part = static_cast<float*>(a->workspace_dev); p.err = ctx->err_dev;
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  const unsigned grid = static_cast<unsigned>(a->batch) * a->rows * a->heads;
-  if (a->cache.head_dim == 128) {
-    if (p.bf16) kv4_attn_simple<128, __nv_bfloat16><<<grid, 128, 0, s>>>(p);
-    else kv4_attn_simple<128, __half><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (p.bf16) kv4_attn_simple<64, __nv_bfloat16><<<grid, 128, 0, s>>>(p);
-    else kv4_attn_simple<64, __half><<<grid, 128, 0, s>>>(p);
-  }
-  AGXC_CUDA(cudaGetLastError());
-  return 0;
+  const bool bf16 = a->dtype == AGXC_BF16;
+  if (a->cache.head_dim == 128)
+    return bf16 ? attn_launch_nt<128, __nv_bfloat16>(p, sh.nt, s) : attn_launch_nt<128, __half>(p, sh.nt, s);
+  return bf16 ? attn_launch_nt<64, __nv_bfloat16>(p, sh.nt, s) : attn_launch_nt<64, __half>(p, sh.nt, s);
 }
 
 }  // extern "C"
