@@ -12,17 +12,17 @@
 // q is scaled by a power of two a column and the fields' 2^-24 is undone in fp32 (exact). P = p s / sref is rounded to
 // fp16 (11 bits; the only rounding of the pass): sref is the running power of two above the group's scales and the
 // reference m sits 8 below the running maximum, so P stays in fp16's normal range down to 2^-22 of the largest weight.
-// The values' codes are taken about 8 (fields or-ed into 1024 + code, minus 1032: exact) and their bias as b + 8 s, so
+// The values' codes are taken about 8 (a second MMA with the constant -8 in A follows each) and their bias as b + 8 s, so
 // that P's rounding counts by a value's distance from its group's middle and the sums over thousands of keys stay
 // small beside what the tensor core's accumulation drops (codes of one sign: 3.6e-4 off at 8,192 keys, 2-norm; about 8:
 // 2.8e-4, of which the output's own fp16 rounding is 2.1e-4). m and sref move only when a score passes m + 12 or a
 // scale passes 8 sref (one vote for 32 keys), which rescales the accumulators.
 //
-// Split. The 32-key units of every (sequence, KV head, block of columns) lie end to end; each CTA takes an equal share
-// of that line, whatever the lengths are, and its four warps take its units in turn. A piece that is not a whole item
-// leaves its maximum, sum and values in the workspace, and a second kernel joins the pieces in a fixed order (no
-// atomics: equal calls give equal bits). A warp has two units of shared memory and copies one (a bulk copy a tile, which
-// is contiguous) while it computes on the other.
+// Split. The 128-key blocks of every (sequence, KV head, block of columns) lie end to end; each CTA takes an equal
+// share of that line, whatever the lengths are. A fifth warp copies the blocks, a bulk copy a tile (which is
+// contiguous), into three stages of shared memory, and each of four warps computes on 32 keys of a block. A piece that
+// is not a whole item leaves its maximum, sum and values in the workspace, and a second kernel joins the pieces in a
+// fixed order (no atomics: equal calls give equal bits).
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -31,7 +31,8 @@ namespace agxc {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kThreads = 32 * kWarps;       // of the warps that compute; one more warp copies
+constexpr int kBlock = 32 * kWarps;         // keys a block
 constexpr float kNone = -1e30f;         // the maximum that stands for no key
 
 struct Kv4AttnParams {
@@ -56,10 +57,10 @@ __device__ __forceinline__ int seq_len(const Kv4AttnParams& p, int b) {
   return len;
 }
 
-__device__ __forceinline__ int units_of(int len) { return (len + 31) >> 5; }
+__device__ __forceinline__ int blocks_of(int len) { return (len + kBlock - 1) / kBlock; }
 
-// A CTA's place on the line of units: sequence b, item = kv_head * CB + column block, unit t of its T, and how many
-// units are left of the CTA's share.
+// A CTA's place on the line of blocks: sequence b, item = kv_head * CB + column block, block t of its T, and how many
+// blocks are left of the CTA's share.
 struct Place {
   int b, item, t, T, len;
   long long rem;
@@ -75,21 +76,20 @@ struct Place {
           return;
         }
         len = seq_len(p, b);
-        T = units_of(len);
+        T = blocks_of(len);
       } while (T == 0);
     }
   }
 };
 
-// Units a CTA: the line's length over the CTAs, a multiple of the warps. Every warp computes it for itself.
+// Blocks a CTA: the line's length over the CTAs. Every warp computes it for itself.
 __device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane) {
   long long sum = 0;
-  for (int b = lane; b < p.B; b += 32) sum += units_of(seq_len(p, b));
+  for (int b = lane; b < p.B; b += 32) sum += blocks_of(seq_len(p, b));
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   sum *= p.c.kvh * p.CB;
-  const long long per = (sum + p.ctas - 1) / p.ctas;
-  return (per + kWarps - 1) / kWarps * kWarps;
+  return (sum + p.ctas - 1) / p.ctas;
 }
 
 // The sequence that holds position `at` of the line, and where its items start.
@@ -100,7 +100,7 @@ __device__ __forceinline__ bool line_find(const Kv4AttnParams& p, int lane, long
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
     const int l = b < p.B ? seq_len(p, b) : 0;
-    const long long mine = static_cast<long long>(units_of(l)) * items;
+    const long long mine = static_cast<long long>(blocks_of(l)) * items;
     long long up = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -119,6 +119,13 @@ __device__ __forceinline__ bool line_find(const Kv4AttnParams& p, int lane, long
   }
   return false;
 }
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// a barrier of the warps that compute
+__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -139,13 +146,6 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
-
-// code - 8 of the even (hi = 0) or 16 (code - 8) of the odd nibble in the low byte of each half of x, in fp16 (exact)
-__device__ __forceinline__ uint32_t about8(uint32_t x, int hi) {
-  const uint32_t u = (x & (hi ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + code, or 1024 + 16 code
-  const __half2 d = __hsub2(as_half2(u), as_half2(hi ? 0x64806480u : 0x64086408u));
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
 
 // D = A B, m16n8k16
 __device__ __forceinline__ void mma_16816_zero(float& d0, float& d1, float& d2, float& d3, uint32_t a0, uint32_t a1,
@@ -192,40 +192,43 @@ __device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float* f) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Shared memory of a CTA: rings [warp][stage] of units, the warps' results [warp][column][hd + 4], {max, sum} of each,
-// barriers and the tiles that were copied [warp][stage].
+// Shared memory of a CTA: stages of a block's tiles, the warps' results [warp][column][hd + 4], {max, sum} of each, the
+// stages' barriers (filled, emptied) and which of their tiles were copied.
 template <int HD, int NT>
 struct Smem {
-  static constexpr int kStages = NT == 1 ? 2 : 3;
-  static constexpr int kStage = 2 * Kv4Tile<HD>::kBytes;
+  static constexpr int kStages = 3;
+  static constexpr int kStage = kBlock / 16 * Kv4Tile<HD>::kBytes;
   static constexpr int kCols = 8 * NT;
   static constexpr int kRow = HD + 4;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kO = kRing;
+  static constexpr int kO = kStages * kStage;
   static constexpr int kMl = kO + kWarps * kCols * kRow * 4;
   static constexpr int kBar = kMl + kWarps * kCols * 8;
-  static constexpr int kCame = kBar + kWarps * kStages * 8;
-  static constexpr int kBytes = kCame + kWarps * kStages * 4;
+  static constexpr int kCame = kBar + 2 * kStages * 8;
+  static constexpr int kBytes = kCame + kStages * 4;
 };
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+__global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
+    kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
   using Tile = Kv4Tile<HD>;
   using Sm = Smem<HD, NT>;
   constexpr int GR = HD / 64;               // groups of 64 dims
   constexpr int S = Sm::kStages, NC = Sm::kCols;
   extern __shared__ __align__(128) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  uint8_t* ring = sm + warp * S * Sm::kStage;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Sm::kBar) + warp * S;
-  volatile unsigned* came = reinterpret_cast<unsigned*>(sm + Sm::kCame) + warp * S;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + Sm::kBar);
+  uint64_t* empty = full + S;
+  volatile unsigned* came = reinterpret_cast<unsigned*>(sm + Sm::kCame);
   float* so = reinterpret_cast<float*>(sm + Sm::kO);
   float2* sml = reinterpret_cast<float2*>(sm + Sm::kMl);
-  if (lane == 0) {
-    for (int i = 0; i < S; ++i) mbar_init(&bar[i], 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
     fence_mbar_init();
   }
-  __syncwarp();
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
@@ -235,77 +238,56 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
     const long long from = quota * blockIdx.x;
     long long start;
     if (quota == 0 || !line_find(p, lane, from, at.b, at.len, start)) return;  // every warp of the CTA alike
-    at.T = units_of(at.len);
+    at.T = blocks_of(at.len);
     const long long off = from - start;
     at.item = static_cast<int>(off / at.T);
     at.t = static_cast<int>(off % at.T);
     at.rem = quota;
   }
-  const int tiles_page = p.c.page >> 4;
-  // where the units end that some column of the item's block sees
+  // where the blocks end that some column of the item's column block sees
   auto seen = [&](const Place& w) {
     const int last = min(p.n - 1, (w.item % p.CB * NC + NC - 1) / p.G);
     const int keys = w.len - p.n + last + 1;
-    return keys > 0 ? min(w.end(), units_of(keys)) : 0;
+    return keys > 0 ? min(w.end(), blocks_of(keys)) : 0;
   };
 
-  // The warp's copies run S units ahead of its reads; `ahead` walks the line on its own. Lanes 0 and 1 look after the
-  // unit's first and second tile: the page (fetched a unit early) and the tile's place in it.
-  Place ahead = at;
-  int a_unit, a_end, a_slot = 0, flying = 0, a_page = -1, a_in = 0, a_idx = 0, a_tiles = 0;
-  const int32_t* a_row = nullptr;
-  const uint8_t* a_head = nullptr;
-  bool dead = false, more = true;
-  auto enter = [&]() {  // the warp's first unit of the place `ahead` has come to
-    a_unit = ahead.t + warp;
-    a_end = seen(ahead);
-    const int tile = 2 * a_unit + (lane & 1);
-    a_idx = tile / tiles_page;
-    a_in = tile % tiles_page;
-    a_tiles = (ahead.len + 15) >> 4;
-    a_row = p.table + static_cast<long long>(ahead.b) * p.table_ld;
-    a_head = p.c.data + static_cast<size_t>(ahead.item / p.CB) * tiles_page * Tile::kBytes;
-  };
-  auto settle = [&]() {  // the next unit that exists, and its pages
-    while (a_unit >= a_end) {
-      ahead.next(p);
-      if (ahead.rem <= 0) {
-        more = false;
-        return;
+  if (warp == kWarps) {  // the copies: lane x looks after tile x of each block
+    const int tiles_page = p.c.page >> 4;
+    unsigned uses = 0;
+    int stage = 0;
+    bool dead = false;
+    for (; at.rem > 0 && !dead; at.next(p)) {
+      const int tiles = (at.len + 15) >> 4, end = seen(at);
+      const int32_t* row = p.table + static_cast<long long>(at.b) * p.table_ld;
+      for (int blk = at.t; blk < end; ++blk) {
+        const int tile = blk * (kBlock / 16) + lane;
+        const bool mine = lane < kBlock / 16 && tile < tiles;
+        const int page = mine ? __ldg(row + tile / tiles_page) : -1;
+        const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(p.c.pages);
+        if (mine && !ok) atomicOr(p.err, kErrBadPos);
+        const unsigned mask = __ballot_sync(0xffffffffu, ok);
+        if (uses >= S && !mbar_wait_quiet(&empty[stage], uses / S - 1 & 1, p.err)) {
+          dead = true;
+          break;
+        }
+        if (lane == 0) {
+          came[stage] = mask;
+          mbar_arrive_expect_tx(&full[stage], __popc(mask) * Tile::kBytes);
+        }
+        __syncwarp();
+        if (ok)
+          bulk_g2s(sm + stage * Sm::kStage + lane * Tile::kBytes, Tile::ptr(p.c, page, at.item / p.CB, tile % tiles_page),
+                   Tile::kBytes, &full[stage]);
+        stage = stage + 1 == S ? 0 : stage + 1;
+        ++uses;
       }
-      enter();
     }
-    if (lane < 2 && 2 * a_unit + lane < a_tiles) a_page = __ldg(a_row + a_idx);
-  };
-  const size_t page_bytes = static_cast<size_t>(p.c.kvh) * tiles_page * Tile::kBytes;
-  auto issue = [&]() {
-    if (!more || dead) return;
-    const bool mine = lane < 2 && 2 * a_unit + lane < a_tiles;
-    const bool ok = mine && static_cast<unsigned>(a_page) < static_cast<unsigned>(p.c.pages);
-    if (mine && !ok) atomicOr(p.err, kErrBadPos);
-    const unsigned mask = __ballot_sync(0xffffffffu, ok);
-    if (lane == 0) {
-      came[a_slot] = mask;
-      mbar_arrive_expect_tx(&bar[a_slot], __popc(mask) * Tile::kBytes);
-    }
-    __syncwarp();
-    if (ok)
-      bulk_g2s(ring + a_slot * Sm::kStage + lane * Tile::kBytes, a_head + a_page * page_bytes + a_in * Tile::kBytes,
-               Tile::kBytes, &bar[a_slot]);
-    a_slot = a_slot + 1 == S ? 0 : a_slot + 1;
-    ++flying;
-    a_unit += kWarps;
-    a_in += 2 * kWarps;
-    while (a_in >= tiles_page) {
-      a_in -= tiles_page;
-      ++a_idx;
-    }
-    settle();
-  };
-  enter();
-  settle();
-  for (int i = 0; i < S; ++i) issue();
+    // every copy lands before the CTA's memory is another's
+    for (unsigned x = uses < S ? 0 : uses - S; x < uses; ++x) mbar_wait_quiet(&full[x % S], x / S & 1, p.err);
+    return;
+  }
 
+  bool dead = false;                        // a wait gave up: the error word says so, and nothing more is computed
   int slot = 0, phase = 0;
   while (at.rem > 0) {
     const int j = at.item / p.CB, col0 = at.item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
@@ -388,13 +370,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
     }
 
     const int end = seen(at);
-    bool fresh = true;                       // no key yet: m is set, up or down, by the first unit
-    for (int unit = at.t + warp; unit < end; unit += kWarps) {
-      if (!dead && !mbar_wait_bounded(&bar[slot], phase, p.err)) dead = true;
+    bool fresh = true;                       // no key yet: m is set, up or down, by the first ones
+    for (int blk = at.t; blk < end; ++blk) {
+      if (!dead && !mbar_wait_bounded(&full[slot], phase, p.err)) dead = true;
       if (dead) continue;
-      --flying;
-      const unsigned mask = came[slot];
-      const uint8_t* st = ring + slot * Sm::kStage;
+      const unsigned mask = came[slot] >> (2 * warp) & 3u;
+      const uint8_t* st = sm + slot * Sm::kStage + warp * 2 * Tile::kBytes;
+      const int key0 = blk * kBlock + warp * 32;
+      if (mask != 0u) {
       float y[2][NT][4];                     // log2 of the weights of (key r, columns 2c, 2c + 1), (key r + 8, the same)
       uint32_t ve[2][2][GR];                 // V's {scale, bias} of keys r, r + 8
       bool move = fresh;
@@ -418,21 +401,22 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
           }
         }
         float d[NT][GR][4];
+        // the groups' chains of four in turn, so that an MMA does not wait for the one before it
 #pragma unroll
-        for (int g = 0; g < GR; ++g)
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t a = kw[0][2 * g + w], b = kw[1][2 * g + w], a8 = a >> 8, b8 = b >> 8;
-            const uint32_t f0 = a & 0x000f000fu, f1 = b & 0x000f000fu, f2 = a & 0x00f000f0u, f3 = b & 0x00f000f0u;
-            const uint32_t e0 = a8 & 0x000f000fu, e1 = b8 & 0x000f000fu, e2 = a8 & 0x00f000f0u, e3 = b8 & 0x00f000f0u;
+          for (int up = 0; up < 2; ++up)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float* x = d[nt][g];
-              if (w == 0) mma_16816_zero(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][0], qf[nt][g][w][1]);
-              else mma_16816(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][0], qf[nt][g][w][1]);
-              mma_16816(x[0], x[1], x[2], x[3], e0, e1, e2, e3, qf[nt][g][w][2], qf[nt][g][w][3]);
+            for (int g = 0; g < GR; ++g) {
+              const uint32_t a = kw[0][2 * g + w] >> (8 * up), b = kw[1][2 * g + w] >> (8 * up);
+              const uint32_t f0 = a & 0x000f000fu, f1 = b & 0x000f000fu, f2 = a & 0x00f000f0u, f3 = b & 0x00f000f0u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float* x = d[nt][g];
+                if (w + up == 0) mma_16816_zero(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][0][0], qf[nt][g][0][1]);
+                else mma_16816(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][2 * up], qf[nt][g][w][2 * up + 1]);
+              }
             }
-          }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float2 sb[GR];
@@ -450,12 +434,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
             }
         }
       }
-      if (unit * 32 + 32 > least || mask != 3u) {  // the mask's edge: an unseen key weighs nothing, whatever its bytes hold
+      if (key0 + 32 > least || mask != 3u) {  // the mask's edge: an unseen key weighs nothing, whatever its bytes hold
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int key = mask >> h & 1 ? unit * 32 + h * 16 + r + 8 * i : 0x7fffffff;
+            const int key = mask >> h & 1 ? key0 + h * 16 + r + 8 * i : 0x7fffffff;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -478,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
         big[g] = __low2float(__hmax2(a, b));
         move |= big[g] > 8.f * sref[g];
       }
-      if (mask != 0u && __any_sync(0xffffffffu, move)) {
+      if (__any_sync(0xffffffffu, move)) {
         float fg[GR];
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
@@ -494,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
             float mx = fmaxf(fmaxf(y[0][nt][e], y[0][nt][2 + e]), fmaxf(y[1][nt][e], y[1][nt][2 + e]));
 #pragma unroll
             for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            // the reference goes up by this much; a column that sees none of the first unit's keys sees no later ones
+            // the reference goes up by this much; a column that sees none of the first keys sees no later ones
             const float by = fresh ? (mx > -INFINITY ? mx - 8.f : 0.f) : fmaxf(0.f, mx - 8.f);
             const float f = fresh ? 1.f : ex2(-by);
             m[nt][e] += by;
@@ -515,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
             }
           }
       }
-      if (mask != 0u) fresh = false;
+      fresh = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // weights: P operands, the sum, and the bias term
@@ -561,17 +545,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
           const uint32_t ya = prmt(vw[0][g], vw[1][g], 0x7632u), yb = prmt(vw[2][g], vw[3][g], 0x7632u);
           const uint32_t a[4] = {xa, xa >> 8, ya, ya >> 8}, b[4] = {xb, xb >> 8, yb, yb >> 8};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t a0 = about8(a[k], 0), a1 = about8(a[k], 1), a2 = about8(b[k], 0), a3 = about8(b[k], 1);
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_16816(o[nt][g][k][0], o[nt][g][k][1], o[nt][g][k][2], o[nt][g][k][3], a0, a1, a2, a3, pf[nt][g][0],
+            for (int nt = 0; nt < NT; ++nt) {
+              float* x = o[nt][g][k];
+              mma_16816(x[0], x[1], x[2], x[3], a[k] & 0x000f000fu, a[k] & 0x00f000f0u, b[k] & 0x000f000fu,
+                        b[k] & 0x00f000f0u, pf[nt][g][0], pf[nt][g][1]);
+            }
+          // -8 as the fields have it: 8 and 16 x 8 steps of 2^-24 below zero
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float* x = o[nt][g][k];
+              mma_16816(x[0], x[1], x[2], x[3], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][g][0],
                         pf[nt][g][1]);
-          }
+            }
         }
       }
-      __syncwarp();                        // every lane has read the unit: the next copy may overwrite it
-      issue();
+      }
+      __syncwarp();                        // every lane has read its keys: the next copy may overwrite them
+      if (lane == 0) mbar_arrive(&empty[slot]);
       slot = slot + 1 == S ? 0 : slot + 1;
       if (slot == 0) phase ^= 1;
     }
@@ -591,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
           float bias = bt[nt][g][e];
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) bias += __shfl_xor_sync(0xffffffffu, bias, x);
-          const float f0 = sref[g], f1 = 0.0625f * sref[g];
+          const float f0 = 16777216.f * sref[g], f1 = 1048576.f * sref[g];
           float* dst = so + (warp * NC + col) * Sm::kRow + 64 * g + 8 * r;
           *reinterpret_cast<float4*>(dst) =
               make_float4(fmaf(o[nt][g][0][e], f0, bias), fmaf(o[nt][g][0][2 + e], f1, bias),
@@ -601,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
                           fmaf(o[nt][g][3][e], f0, bias), fmaf(o[nt][g][3][2 + e], f1, bias));
         }
       }
-    __syncthreads();
+    warps_sync();
     // the four warps joined; whole items are written out, pieces go to the workspace
     const bool whole = at.t == 0 && at.end() == at.T;
     const int piece = 2 * blockIdx.x + (at.t == 0 ? 1 : 0);
@@ -638,16 +632,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv4_attn_kernel(con
         *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
       }
     }
-    __syncthreads();
+    warps_sync();
     at.next(p);
   }
-  // a wait that gave up left copies in flight: they land before the CTA's memory is another's
-  if (dead)
-    for (int i = 0; i < flying; ++i) {
-      mbar_wait_bounded(&bar[slot], phase, p.err);
-      slot = slot + 1 == S ? 0 : slot + 1;
-      if (slot == 0) phase ^= 1;
-    }
 }
 
 // One CTA an item: joins the pieces that the CTAs of kv4_attn_kernel left of it, in their order; writes zeros for a
@@ -658,24 +645,24 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
   const int lane = threadIdx.x & 31;
   const int items = p.c.kvh * p.CB, b = blockIdx.x / items, item = blockIdx.x % items;
   pdl_wait();
-  const int units = units_of(seq_len(p, b));
+  const int blocks = blocks_of(seq_len(p, b));
   const int j = item / p.CB, col0 = item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
   long long c0 = 0, c1 = 0;
-  if (units) {
+  if (blocks) {
     const long long quota = line_quota(p, lane);
     long long before = 0;
-    for (int x = lane; x < b; x += 32) before += units_of(seq_len(p, x));
+    for (int x = lane; x < b; x += 32) before += blocks_of(seq_len(p, x));
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) before += __shfl_xor_sync(0xffffffffu, before, m);
-    const long long start = before * items + static_cast<long long>(item) * units;
+    const long long start = before * items + static_cast<long long>(item) * blocks;
     c0 = start / quota;
-    c1 = (start + units - 1) / quota;
+    c1 = (start + blocks - 1) / quota;
     if (c0 == c1) return;                   // one CTA had all of it
   }
   for (int u = threadIdx.x; u < cols * (HD / 8); u += kThreads) {
     const int col = u / (HD / 8), d = u % (HD / 8) * 8;
     float v[8] = {};
-    if (units) {
+    if (blocks) {
       const float* ml = p.part;
       const float* val = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2;
       float mx = kNone, sum = 0.f;
@@ -719,7 +706,7 @@ int attn_check(const agxc_kv4_attention_args* a) {
 }
 
 // The launch's shape: 16 columns a block where one row's heads do not fill 8, and as many CTAs as the GPU holds at once
-// (four an SM with 8 columns, two with 16), or fewer where the longest lengths possible make fewer than four units each.
+// (three an SM with 8 columns, two with 16), or fewer where the longest lengths possible have fewer blocks.
 struct Shape {
   int nt, cb, ctas;
   int64_t bytes(int hd) const { return static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
@@ -730,11 +717,10 @@ Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   const int64_t cols = static_cast<int64_t>(a->rows) * (a->heads / a->cache.kv_heads);
   s.nt = cols > 8 ? 2 : 1;
   s.cb = static_cast<int>((cols + 8 * s.nt - 1) / (8 * s.nt));
-  const int64_t units = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb *
-                        ((static_cast<int64_t>(a->max_pages) * a->cache.page_size + 31) / 32);
-  const int64_t full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 4 : 2);
-  const int64_t want = (units + kWarps - 1) / kWarps;
-  s.ctas = static_cast<int>(want < 1 ? 1 : want < full ? want : full);
+  const int64_t blocks = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb *
+                        ((static_cast<int64_t>(a->max_pages) * a->cache.page_size + kBlock - 1) / kBlock);
+  const int64_t full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
+    s.ctas = static_cast<int>(blocks < 1 ? 1 : blocks < full ? blocks : full);
   return s;
 }
 
@@ -748,7 +734,7 @@ int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
     AGXC_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     allowed[dev] = true;
   }
-  if (int rc = launch_ex(kv4_attn_kernel<HD, NT, T>, dim3(p.ctas), dim3(kThreads), smem, s, 1, p)) return rc;
+  if (int rc = launch_ex(kv4_attn_kernel<HD, NT, T>, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
   return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(kThreads), 0, s,
                    1, p);
 }
