@@ -10,10 +10,10 @@
 //   1  the maximum (its first index is a greedy row's token) and the least finite logit
 //   2  top-k: counts in 1,024 bins, equal steps of the logit down to weight zero or the least logit; the bin that holds
 //      rank k. Up to 2,048 elements in that bin and above go to one CTA as a list; it sorts them and finishes the row
-//   3  top-p: the same with the bins' exact weights (64 bits as two 32-bit shared-memory adds, the second with the
-//      first's carry)
-//   4  more than a list: only the bin of the cut is listed and sorted, to find the key it falls on; a bin that is more
-//      than a list (thousands of equal logits) is cut bit by bit instead
+//   3  top-p: the bins' exact weights (64 bits as two 32-bit shared-memory adds, the second with the first's carry, rarely
+//      needed); the bin that holds the bar
+//   4  where a bin holds a cut, only that bin is listed and sorted, to find the key it falls on; a bin that is more than
+//      a list (thousands of equal logits) is cut bit by bit instead
 //   5  the kept weights' total and the token, in index order: the warp, then the element, that the target falls on
 #include <cooperative_groups.h>
 
@@ -32,7 +32,7 @@ constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 struct SampleParams {
   const void* x;
   int64_t ld;
-  int B, V, per, cached;  // per = elements of a CTA, cached = how many of them shared memory holds
+  int B, V, per, cached;  // per = elements of a CTA, cached = how many of them shared memory holds (a multiple of 16)
   const float* u;
   float T, top_p, min_p;
   int top_k;
@@ -42,29 +42,41 @@ struct SampleParams {
   const float* m_a;
   int32_t* token;
   float* prob;
+  unsigned* err;
 };
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 2048, kMaxCluster = 16;
 
+constexpr int kCopies = 4;  // pieces that a CTA's range is copied in: the first is looked at while the last are on their way
+
 template <int DT>
-__device__ __forceinline__ float as_logit(uint32_t bits) {  // NaN ranks as -inf, the two zeros alike
-  float v;
-  if (DT == AGXC_F32) v = __uint_as_float(bits);
-  else if (DT == AGXC_F16) v = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-  else v = __uint_as_float(bits << 16);
-  return v != v ? -INFINITY : v + 0.f;
+__device__ __forceinline__ float as_float(uint32_t bits) {
+  if (DT == AGXC_F32) return __uint_as_float(bits);
+  if (DT == AGXC_F16) return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  return __uint_as_float(bits << 16);
 }
 
 template <int DT>
-__device__ __forceinline__ float logit(const void* x, int64_t i) {
-  return DT == AGXC_F32 ? as_logit<DT>(static_cast<const uint32_t*>(x)[i])
-                        : as_logit<DT>(static_cast<const unsigned short*>(x)[i]);
-}
+struct Raw {
+  using Type = uint32_t;
+};
+template <>
+struct Raw<AGXC_F16> {
+  using Type = uint16_t;
+};
+template <>
+struct Raw<AGXC_BF16> {
+  using Type = uint16_t;
+};
+template <int DT>
+constexpr uint32_t kNaN = DT == AGXC_F32 ? 0x7FFFFFFFu : 0x7FFFu;
+template <int DT>
+constexpr uint32_t kMinusInf = DT == AGXC_F32 ? 0xFF800000u : DT == AGXC_F16 ? 0xFC00u : 0xFF80u;
 
 // larger logits first, then lower indices: the larger key ranks first
 __device__ __forceinline__ uint64_t rank_key(float v, int i) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.f);  // the two zeros rank alike
   const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
   return static_cast<uint64_t>(o) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i));
 }
@@ -81,34 +93,42 @@ __device__ __forceinline__ uint64_t weight(float e) {
   return up >= 0 ? static_cast<uint64_t>(m) << up : static_cast<uint64_t>(m >> min(-up, 31));
 }
 
-struct Row {
-  float best, inv_t, step;  // step = bins a unit of logit
-  __device__ float down(float v) const { return v == best ? 0.f : __fsub_rn(v, best); }
-  __device__ float e(float v) const { return v == -INFINITY ? 0.f : expf(__fmul_rn(down(v), inv_t)); }
-  // -inf weighs nothing and is in none
-  __device__ int bin(float v) const {
-    return v == -INFINITY ? kBins : min(kBins - 1, __float2int_rz(-down(v) * step));
+// A sum of weights from their fp32 exps, 20 bits at a time: 8 + e rounded towards zero has floor(2^20 e) in its low bits,
+// and 2^-17 plus what that leaves has the next 20. The constants' own bits are taken off by the count (at most 4,095).
+struct WeightSum {
+  uint32_t hi = 0, lo = 0, n = 0;
+  __device__ void add(float e) {
+    const float t = __fadd_rz(e, 8.f), u = __fadd_rz(__fsub_rn(e, __fsub_rn(t, 8.f)), 7.62939453125e-6f);
+    hi += __float_as_uint(t);
+    lo += __float_as_uint(u);
+    ++n;
+  }
+  __device__ uint64_t get() const {
+    return (static_cast<uint64_t>(hi - n * 0x41000000u) << 20) + (lo - n * 0x37000000u);
   }
 };
 
-struct Best {
-  float v, least;
-  int i;
+struct Row {
+  float best, inv_t, step;  // step = bins a unit of logit
+  __device__ float e(float v) const { return expf(__fmul_rn(__fsub_rn(v, best), inv_t)); }
+  __device__ float place(float v) const { return fminf(__fmul_rn(__fsub_rn(best, v), step), kBins - 1.f); }  // bin = its floor
 };
 
 struct Shared {
-  Best best;
+  float2 best;  // {largest, least}
   uint64_t sum[2];
-  int n_list, bin;
+  uint64_t copied[kCopies];
+  int n_list, bin, first;
   uint64_t before, total, cut;
   uint64_t warp64[kWarps];
   uint64_t warp_kept[kWarps];
-  Best warp_best[kWarps];
   alignas(16) uint32_t count[kBins];
   alignas(16) uint32_t lo[kBins];
   alignas(16) uint32_t hi[kBins];
   uint64_t list[kList];
 };
+
+__device__ __forceinline__ int bin_of(float place) { return __float_as_int(__fadd_rz(place, 8388608.f)) - 0x4B000000; }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -182,126 +202,242 @@ __device__ __forceinline__ uint64_t target_of(float u, uint64_t total) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
+  using T16 = typename Raw<DT>::Type;
+  constexpr int kSize = sizeof(T16);
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(dyn);
-  float* cache = reinterpret_cast<float*>(dyn + align16(sizeof(Shared)));
+  T16* cache = reinterpret_cast<T16*>(dyn + align16(sizeof(Shared)));
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x / C;
   const int64_t base = static_cast<int64_t>(b) * p.ld;
-  const int i0 = min(p.V, rank * p.per), n = min(p.V, i0 + p.per) - i0, nc = min(n, p.cached);
-  const float T = p.T_a ? p.T_a[b] : p.T, top_p = p.p_a ? p.p_a[b] : p.top_p, min_p = p.m_a ? p.m_a[b] : p.min_p;
+  const int r0 = min(p.V, rank * p.per), n = min(p.V, r0 + p.per) - r0;
+  // The range lies at `pad` in the CTA's space, so that its first 16-byte boundary is one there too; places before and
+  // after it hold NaN, then -inf. Everything goes by fours of places; index = place + i0.
+  const T16* src = static_cast<const T16*>(p.x) + base + r0;
+  const int to16 = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / kSize;
+  const int pad = (16 / kSize - to16) % (16 / kSize), i0 = r0 - pad, quads = (pad + n + 3) / 4;
+  const int nc = min(n, p.cached - pad), head = min(nc, to16), bulk = (nc - head) / (16 / kSize) * (16 / kSize);
+
+  // 1: the range into shared memory: bulk copies of its aligned middle, plain loads at its ends
+  if (tid == 0) {
+    for (int c = 0; c < kCopies; ++c) mbar_init(&sh.copied[c], 1);
+    fence_mbar_init();
+    const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;
+    for (int c = 0; c < kCopies; ++c) {
+      const int at = min(bulk, c * each), len = min(bulk, at + each) - at;
+      mbar_arrive_expect_tx(&sh.copied[c], len * kSize);
+      if (len) bulk_g2s(cache + pad + head + at, src + head + at, len * kSize, &sh.copied[c]);
+    }
+  }
+  if (tid < 16) {
+    if (tid < pad) cache[tid] = static_cast<T16>(kNaN<DT>);
+    if (tid < head) cache[pad + tid] = src[tid];
+    const int tail = head + bulk + tid;  // fewer than 16 bytes of the range, then fewer than four places
+    if (tail < nc) cache[pad + tail] = src[tail];
+    else if (nc == n && pad + tail < 4 * quads) cache[pad + tail] = static_cast<T16>(kNaN<DT>);
+  }
+  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.lo[x] = sh.hi[x] = 0;
+  if (tid == 0) sh.n_list = 0, sh.first = 0x7fffffff;
+  const float T = fminf(p.T_a ? p.T_a[b] : p.T, FLT_MAX), top_p = p.p_a ? p.p_a[b] : p.top_p,
+              min_p = p.m_a ? p.m_a[b] : p.min_p;
   const int k_in = p.k_a ? p.k_a[b] : p.top_k;
   const bool use_k = k_in > 0 && k_in < p.V, use_p = top_p < 1.f;
-
-  // 1: the range into shared memory, 16 bytes at a time from its first 16-byte boundary
-  constexpr int kSize = DT == AGXC_F32 ? 4 : 2, kVec = 16 / kSize;
-  const uint8_t* src = static_cast<const uint8_t*>(p.x) + (base + i0) * kSize;
-  const int head = min(nc, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / kSize);
-  cache += (4 - head % 4) % 4;
-  Best mine = {-INFINITY, INFINITY, 0x7fffffff};
-  auto see = [&](float v, int i) {
-    if (v > mine.v || mine.i == 0x7fffffff) mine.v = v, mine.i = i;
-    if (v > -INFINITY) mine.least = fminf(mine.least, v);
-  };
-  if (tid < head) {
-    const float v = logit<DT>(p.x, base + i0 + tid);
-    cache[tid] = v;
-    see(v, i0 + tid);
-  }
-  const int vecs = (nc - head) / kVec;
-#pragma unroll 4
-  for (int x = tid; x < vecs; x += kThreads) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + head * kSize) + x);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float f[kVec];
-#pragma unroll
-    for (int y = 0; y < kVec; ++y)
-      f[y] = kSize == 4 ? as_logit<DT>(u[y & 3]) : as_logit<DT>(u[y / 2] >> (16 * (y & 1)) & 0xffffu);
-    const int at = head + x * kVec;
-#pragma unroll
-    for (int y = 0; y < kVec; y += 4) *reinterpret_cast<float4*>(cache + at + y) = make_float4(f[y], f[y + 1], f[y + 2], f[y + 3]);
-#pragma unroll
-    for (int y = 0; y < kVec; ++y) see(f[y], i0 + at + y);
-  }
-  for (int x = head + vecs * kVec + tid; x < n; x += kThreads) {
-    const float v = logit<DT>(p.x, base + i0 + x);
-    if (x < nc) cache[x] = v;
-    see(v, i0 + x);
-  }
-  auto get = [&](int x) { return x < nc ? cache[x] : logit<DT>(p.x, base + i0 + x); };
-  auto join = [](Best& a, float v, float least, int i) {
-    if (v > a.v || (v == a.v && i < a.i)) a.v = v, a.i = i;
-    a.least = fminf(a.least, least);
-  };
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1)
-    join(mine, __shfl_xor_sync(0xffffffffu, mine.v, m), __shfl_xor_sync(0xffffffffu, mine.least, m),
-         __shfl_xor_sync(0xffffffffu, mine.i, m));
-  if (lane == 0) sh.warp_best[warp] = mine;
-  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.lo[x] = sh.hi[x] = 0;
-  if (tid == 0) sh.n_list = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) join(mine, sh.warp_best[w].v, sh.warp_best[w].least, sh.warp_best[w].i);
-    sh.best = mine;
+
+  bool has_inf = false;  // the row's maximum is +inf
+  // four places' logits; NaN ranks as -inf, and beside +inf everything does
+  auto get4 = [&](int q, float* f) {
+    if (4 * q + 3 < p.cached) {
+      if constexpr (kSize == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(cache + 4 * q);
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(cache + 4 * q);
+        f[0] = as_float<DT>(v.x & 0xffffu); f[1] = as_float<DT>(v.x >> 16);
+        f[2] = as_float<DT>(v.y & 0xffffu); f[3] = as_float<DT>(v.y >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int x = 4 * q + y - pad;
+        f[y] = x >= 0 && x < n ? as_float<DT>(src[x]) : -INFINITY;
+        if (f[y] != f[y]) f[y] = -INFINITY;
+        if (has_inf) f[y] = f[y] == INFINITY ? 0.f : -INFINITY;
+      }
+    }
+  };
+  auto put = [&](int x, float v) {  // a special value
+    if (x < p.cached) cache[x] = DT == AGXC_F32 ? static_cast<T16>(__float_as_uint(v))
+                                                : static_cast<T16>(v == 0.f ? 0u : kMinusInf<DT>);
+  };
+  float best = -INFINITY, least = INFINITY;
+  int seen = 0;  // copies that have landed
+  for (int q = tid; q < quads; q += kThreads) {
+    const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;
+    while (seen < kCopies && seen * each < 4 * q + 4 - pad - head) mbar_wait_bounded(&sh.copied[seen++], 0, p.err);
+    float f[4];
+    get4(q, f);
+    best = fmaxf(fmaxf(best, fmaxf(f[0], f[1])), fmaxf(f[2], f[3]));
+    least = fminf(fminf(least, fminf(f[0], f[1])), fminf(f[2], f[3]));
+    if (f[0] != f[0] || f[1] != f[1] || f[2] != f[2] || f[3] != f[3]) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (f[y] != f[y]) {
+          put(4 * q + y, -INFINITY);
+          if (4 * q + y >= pad && 4 * q + y < pad + n) least = -INFINITY;
+        }
+    }
+  }
+  while (seen < kCopies) mbar_wait_bounded(&sh.copied[seen++], 0, p.err);
+  best = warp_max(best);
+  least = -warp_max(-least);
+  if (lane == 0) reinterpret_cast<float2*>(sh.warp64)[warp] = make_float2(best, least);
+  __syncthreads();
+  if (warp == 0) {
+    const float2 o = lane < kWarps ? reinterpret_cast<float2*>(sh.warp64)[lane] : make_float2(-INFINITY, INFINITY);
+    best = warp_max(o.x);
+    least = -warp_max(-o.y);
+    if (lane == 0) sh.best = make_float2(best, least);
   }
   cluster.sync();
-  mine = {-INFINITY, INFINITY, 0x7fffffff};
-  for (int c = 0; c < C; ++c) {
-    const Best o = *cluster.map_shared_rank(&sh.best, c);
-    join(mine, o.v, o.least, o.i);
+  {
+    const float2 o = lane < C ? *cluster.map_shared_rank(&sh.best, lane) : make_float2(-INFINITY, INFINITY);
+    best = warp_max(o.x);
+    least = -warp_max(-o.y);
   }
-  if (mine.v == -INFINITY || T == 0.f) {
-    if (rank == 0 && tid == 0) {
-      const bool none = mine.v == -INFINITY || !(1.f >= min_p);
-      p.token[b] = none ? -1 : mine.i;
-      if (p.prob) p.prob[b] = none ? 0.f : 1.f;
+  if (best == -INFINITY || T == 0.f) {  // nothing finite, or greedy: the first maximum
+    const bool none = best == -INFINITY || !(1.f >= min_p);
+    if (!none) {
+      int first = 0x7fffffff;
+      for (int q = tid; q < quads && first == 0x7fffffff; q += kThreads) {
+        float f[4];
+        get4(q, f);
+#pragma unroll
+        for (int y = 3; y >= 0; --y)
+          if (f[y] == best) first = i0 + 4 * q + y;
+      }
+      if (first != 0x7fffffff) atomicMin(cluster.map_shared_rank(&sh.first, 0), first);
     }
     cluster.sync();
+    if (rank == 0 && tid == 0) {
+      p.token[b] = none ? -1 : sh.first;
+      if (p.prob) p.prob[b] = none ? 0.f : 1.f;
+    }
     return;
   }
+  if (best == INFINITY) {
+    for (int q = tid; q < quads; q += kThreads) {
+      float f[4];
+      get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) put(4 * q + y, f[y] == INFINITY ? 0.f : -INFINITY);
+    }
+    __syncthreads();
+    has_inf = true;
+    best = 0.f;
+    least = least == INFINITY ? 0.f : -INFINITY;
+  }
   Row r;
-  r.best = mine.v;
+  r.best = best;
   r.inv_t = __fdiv_rn(1.f, T);
   const float zero_at = 28.f * T;  // 2^40 e^-28 < 1: weights are zero from here down
-  const bool zero_last = mine.v - mine.least >= zero_at;
-  const float range = zero_last ? zero_at : mine.v - mine.least;
-  r.step = range > 0.f ? (kBins - 1) / range : 0.f;
-  const int ends = zero_last ? kBins - 1 : kBins;  // bins from here on weigh nothing
+  const bool zero_last = best - least >= zero_at;
+  const float range = zero_last ? zero_at : best - least;
+  r.step = range > 1e-30f ? (kBins - 1) / range : 0.f;
+  const float ends = zero_last ? kBins - 1.f : kBins;  // places from here on weigh nothing
 
   int round = 0;
   auto cluster_sum = [&](uint64_t v) {  // over the row, on every thread
     v = block_sum(v, sh.warp64);
     if (tid == 0) sh.sum[round] = v;
     cluster.sync();
-    uint64_t t = 0;
-    for (int c = 0; c < C; ++c) t += *cluster.map_shared_rank(&sh.sum[round], c);
+    const uint64_t t = warp_sum64(lane < C ? *cluster.map_shared_rank(&sh.sum[round], lane) : 0);
     round ^= 1;
     return t;
   };
-  // elements that pass, as keys, into the first CTA's list (their number is known to fit)
-  auto gather = [&](auto pass) {
+  // elements at places from `lo` to below `hi` whose keys reach `from`, as keys, into the first CTA's list; returns how
+  // many there are (the list holds the first kList of them)
+  auto gather = [&](float lo, float hi, uint64_t from) {
     uint64_t* list = cluster.map_shared_rank(sh.list, 0);
     int* count = cluster.map_shared_rank(&sh.n_list, 0);
-    for (int x0 = warp * 32; x0 < n; x0 += kThreads) {
-      const int x = x0 + lane;
-      const float v = x < n ? get(x) : -INFINITY;
-      const bool in = x < n && pass(v, i0 + x);
-      const unsigned some = __ballot_sync(0xffffffffu, in);
-      if (!some) continue;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(count, __popc(some));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(some & ((1u << lane) - 1));
-      if (in && at < kList) list[at] = rank_key(v, i0 + x);
+    for (int q0 = warp * 32; q0 < quads; q0 += kThreads) {
+      const int q = q0 + lane;
+      float f[4];
+      bool in[4], any = false;
+      if (q < quads) get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float at = q < quads ? r.place(f[y]) : -1.f;
+        in[y] = at >= lo && at < hi && f[y] > -INFINITY && (!from || rank_key(f[y], i0 + 4 * q + y) >= from);
+        any |= in[y];
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const unsigned some = __ballot_sync(0xffffffffu, in[y]);
+        if (!some) continue;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(count, __popc(some));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(some & ((1u << lane) - 1));
+        if (in[y] && at < kList) list[at] = rank_key(f[y], i0 + 4 * q + y);
+      }
     }
     cluster.sync();
+    return *cluster.map_shared_rank(&sh.n_list, 0);
   };
-  // the first CTA has every candidate in its list: cut, draw, done
+  auto tell = [&](int token, uint64_t w, uint64_t total) {
+    p.token[b] = token;
+    if (p.prob)
+      p.prob[b] = total ? static_cast<float>(__ddiv_rn(__ll2double_rn(static_cast<long long>(w)),
+                                                       __ll2double_rn(static_cast<long long>(total)))) : 0.f;
+  };
+  // The first CTA has every candidate in its list: cut, draw, done. Up to 128 candidates are ranked by comparing each
+  // with all (four threads a candidate); more are sorted, and the token is found by two histograms over the index.
   auto finish_list = [&](int len, int keep) {
-    if (rank == 0) {
+    if (rank == 0 && len <= kThreads / 4) {
+      const int x = tid >> 2;
+      const uint64_t key = x < len ? sh.list[x] : 0;
+      const float e = x < len ? r.e(key_logit(key)) : 0.f;
+      if (x < len && (tid & 3) == 0) sh.list[kList / 2 + x] = weight(e);
+      __syncthreads();
+      int ahead = 0;
+      uint64_t before = 0, total = 0;
+      for (int y = tid & 3; y < len; y += 4) {
+        const uint64_t o = sh.list[y];
+        if (o > key) {
+          ++ahead;
+          before += sh.list[kList / 2 + y];
+        }
+      }
+#pragma unroll
+      for (int m = 1; m <= 2; m <<= 1) {
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, m);
+        before += __shfl_xor_sync(0xffffffffu, before, m);
+      }
+      uint64_t w = x < len && ahead < keep ? weight(e) : 0;
+      if (use_p) {
+        total = block_sum((tid & 3) == 0 ? w : 0, sh.warp64);
+        if (before >= top_p_bar(top_p, total)) w = 0;
+      }
+      if (!(e >= min_p)) w = 0;
+      total = block_sum((tid & 3) == 0 ? w : 0, sh.warp64);  // and every thread is past the first weights
+      if (x < len && (tid & 3) == 0) sh.list[kList / 2 + x] = w;
+      __syncthreads();
+      if (total == 0) {
+        if (tid == 0) tell(-1, 0, 0);
+      } else {
+        const uint64_t target = target_of(p.u[b], total);
+        before = 0;
+        for (int y = tid & 3; y < len; y += 4)
+          if (key_index(sh.list[y]) < key_index(key)) before += sh.list[kList / 2 + y];
+#pragma unroll
+        for (int m = 1; m <= 2; m <<= 1) before += __shfl_xor_sync(0xffffffffu, before, m);
+        if ((tid & 3) == 0 && target >= before && target < before + w) tell(key_index(key), w, total);
+      }
+    } else if (rank == 0) {
       sort_list(sh.list, len);
       len = min(len, keep);
       constexpr int kEach = kList / kThreads;
@@ -326,58 +462,95 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       }
       total = block_sum(sum, sh.warp64);
       if (total == 0) {
-        if (tid == 0) {
-          p.token[b] = -1;
-          if (p.prob) p.prob[b] = 0.f;
-        }
+        if (tid == 0) tell(-1, 0, 0);
       } else {
-        const uint64_t target = target_of(p.u[b], total);
-        // the largest index with at most `target` of the weight before it
-        int at = 0;
-        for (int bit = 31 - __clz(p.V); bit >= 0; --bit) {
-          const int to = at | 1 << bit;
-          sum = 0;
+        // the weights over the index in 1,024 steps, then over the indices of the step that the target falls in
+        uint64_t left = target_of(p.u[b], total);
+        int from = 0, each = (p.V + kBins - 1) / kBins;
+        uint64_t w_at = 0;
+        for (int level = 0; level < 2; ++level) {
 #pragma unroll
-          for (int y = 0; y < kEach; ++y)
-            if (w[y] && key_index(sh.list[tid * kEach + y]) < to) sum += w[y];
-          if (block_sum(sum, sh.warp64) <= target) at = to;
-        }
-#pragma unroll
-        for (int y = 0; y < kEach; ++y)
-          if (w[y] && key_index(sh.list[tid * kEach + y]) == at) {
-            p.token[b] = at;
-            if (p.prob)
-              p.prob[b] = static_cast<float>(__ddiv_rn(__ll2double_rn(static_cast<long long>(w[y])),
-                                                       __ll2double_rn(static_cast<long long>(total))));
+          for (int y = 0; y < kEach; ++y) {
+            const int at = w[y] ? (key_index(sh.list[tid * kEach + y]) - from) / each : -1;
+            if (at < 0 || at >= kBins) continue;
+            const uint32_t l = static_cast<uint32_t>(w[y]), old = atomicAdd(&sh.lo[at], l);
+            const uint32_t h = static_cast<uint32_t>(w[y] >> 32) + (old + l < old ? 1u : 0u);
+            if (h) atomicAdd(&sh.hi[at], h);
           }
+          __syncthreads();
+          uint64_t a[2], unused;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) a[y] = static_cast<uint64_t>(sh.hi[2 * tid + y]) << 32 | sh.lo[2 * tid + y];
+          uint64_t at = block_before(a[0] + a[1], sh.warp64, unused);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            sh.lo[2 * tid + y] = sh.hi[2 * tid + y] = 0;
+            if (left >= at && left < at + a[y]) {
+              sh.bin = 2 * tid + y;
+              sh.before = at;
+              sh.total = a[y];
+            }
+            at += a[y];
+          }
+          __syncthreads();
+          from += sh.bin * each;
+          left -= sh.before;
+          w_at = sh.total;
+          if (level == 0) {
+            // what is outside the step counts no more
+#pragma unroll
+            for (int y = 0; y < kEach; ++y)
+              if (w[y] && (key_index(sh.list[tid * kEach + y]) < from || key_index(sh.list[tid * kEach + y]) >= from + each))
+                w[y] = 0;
+            each = 1;
+          }
+          __syncthreads();
+        }
+        if (tid == 0) tell(from, w_at, total);
       }
     }
     cluster.sync();
   };
-  // the key at which `test` of the sum over keys from it up turns true, among the keys of one bin: bit by bit
-  auto bisect = [&](auto sum_from, uint64_t need) {
+  // the largest key from which up a bin's elements sum to `need`, bit by bit
+  auto bisect = [&](auto sum_of, float lo, float hi, uint64_t from, uint64_t need) {
     uint64_t cut = 0;
     for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t at = cut | 1ull << bit;
+      const uint64_t at = cut | 1ull << bit, least_key = at > from ? at : from;
       uint64_t s = 0;
-      for (int x = tid; x < n; x += kThreads) s += sum_from(get(x), i0 + x, at);
+      for (int q = tid; q < quads; q += kThreads) {
+        float f[4];
+        get4(q, f);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float x = r.place(f[y]);
+          if (x >= lo && x < hi && f[y] > -INFINITY && rank_key(f[y], i0 + 4 * q + y) >= least_key) s += sum_of(f[y]);
+        }
+      }
       if (cluster_sum(s) >= need) cut = at;
     }
-    return cut;
+    return cut > from ? cut : from;
   };
 
   uint64_t cut = 0;  // keys from `cut` up are kept
   if (use_k) {
-    for (int x = tid; x < n; x += kThreads) {
-      const int q = r.bin(get(x));
-      if (q < ends) atomicAdd(&sh.count[q], 1u);
+    for (int q = tid; q < quads; q += kThreads) {
+      float f[4];
+      get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float x = r.place(f[y]);
+        if (x < ends && f[y] > -INFINITY) atomicAdd(&sh.count[bin_of(x)], 1u);
+      }
     }
     cluster.sync();
     uint32_t c2[2] = {};
-    for (int c = 0; c < C; ++c) {
-      const uint2 o = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, c) + 2 * tid);
-      c2[0] += o.x; c2[1] += o.y;
-    }
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < C) {
+        const uint2 o = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, c) + 2 * tid);
+        c2[0] += o.x;
+        c2[1] += o.y;
+      }
     uint64_t all;
     uint64_t below = block_before(static_cast<uint64_t>(c2[0]) + c2[1], sh.warp64, all);
     if (all <= static_cast<uint64_t>(k_in) && all <= kList && !use_p) {
@@ -398,54 +571,52 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       const int bin = sh.bin;
       const uint64_t before = sh.before, through = bin < 0 ? all : sh.total;
       if (through <= kList) {
-        gather([&](float v, int) { const int q = r.bin(v); return q < ends && (bin < 0 || q <= bin); });
+        gather(0.f, bin < 0 ? ends : bin + 1.f, 0);
         finish_list(static_cast<int>(through), k_in);
         return;
       }
       if (bin >= 0) {
-        const int left = static_cast<int>(k_in - before);
+        const uint64_t left = k_in - before;
         if (through - before <= kList) {
-          gather([&](float v, int) { return r.bin(v) == bin; });
+          const int len = gather(static_cast<float>(bin), bin + 1.f, 0);
           if (rank == 0) {
-            sort_list(sh.list, static_cast<int>(through - before));
+            sort_list(sh.list, len);
             if (tid == 0) sh.cut = sh.list[left - 1], sh.n_list = 0;
           }
           cluster.sync();
           cut = *cluster.map_shared_rank(&sh.cut, 0);
         } else {
-          cut = bisect([&](float v, int i, uint64_t at) -> uint64_t { return r.bin(v) == bin && rank_key(v, i) >= at; },
-                       left);
+          cut = bisect([&](float) -> uint64_t { return 1; }, static_cast<float>(bin), bin + 1.f, 0, left);
         }
       }
     }
   }
   if (use_p) {
-    if (use_k) {  // the counts were for top-k
-      cluster.sync();
-      for (int x = tid; x < kBins; x += kThreads) sh.count[x] = 0;
-      __syncthreads();
-    }
-    for (int x = tid; x < n; x += kThreads) {
-      const float v = get(x);
-      const int q = r.bin(v);
-      if (q >= ends || (cut && rank_key(v, i0 + x) < cut)) continue;
-      const uint64_t w = weight(r.e(v));
-      const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&sh.lo[q], l);
-      const uint32_t h = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
-      if (h) atomicAdd(&sh.hi[q], h);
-      atomicAdd(&sh.count[q], 1u);
+    if (use_k) cluster.sync();  // sh.cut has been read
+    for (int q = tid; q < quads; q += kThreads) {
+      float f[4];
+      get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float x = r.place(f[y]);
+        if (!(x < ends && f[y] > -INFINITY) || (cut && rank_key(f[y], i0 + 4 * q + y) < cut)) continue;
+        const uint64_t w = weight(r.e(f[y]));
+        const int at = bin_of(x);
+        const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&sh.lo[at], l);
+        const uint32_t h = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
+        if (h) atomicAdd(&sh.hi[at], h);
+      }
     }
     cluster.sync();
-    uint64_t w2[2] = {}, n2[2] = {};
-    for (int c = 0; c < C; ++c) {
-      const uint2 l = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.lo, c) + 2 * tid);
-      const uint2 h = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.hi, c) + 2 * tid);
-      const uint2 o = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, c) + 2 * tid);
-      w2[0] += static_cast<uint64_t>(h.x) << 32 | l.x;
-      w2[1] += static_cast<uint64_t>(h.y) << 32 | l.y;
-      n2[0] += o.x;
-      n2[1] += o.y;
-    }
+    uint64_t w2[2] = {};
+#pragma unroll 8
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < C) {
+        const uint2 l = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.lo, c) + 2 * tid);
+        const uint2 h = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.hi, c) + 2 * tid);
+        w2[0] += static_cast<uint64_t>(h.x) << 32 | l.x;
+        w2[1] += static_cast<uint64_t>(h.y) << 32 | l.y;
+      }
     uint64_t total;
     uint64_t below = block_before(w2[0] + w2[1], sh.warp64, total);
     const uint64_t bar = top_p_bar(top_p, total);
@@ -454,24 +625,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       if (below < bar && below + w2[y] >= bar) {  // exactly one bin
         sh.bin = 2 * tid + y;
         sh.before = below;
-        sh.total = n2[y];
       }
       below += w2[y];
     }
     __syncthreads();
     const int bin = sh.bin;
-    const uint64_t before = sh.before, in_bin = sh.total;
+    const uint64_t before = sh.before;
+    const int in_bin = gather(static_cast<float>(bin), bin + 1.f, cut);
     if (in_bin <= kList) {
-      const uint64_t from = cut;
-      gather([&](float v, int i) { return r.bin(v) == bin && rank_key(v, i) >= from; });
       if (rank == 0) {
-        sort_list(sh.list, static_cast<int>(in_bin));
+        sort_list(sh.list, in_bin);
         constexpr int kEach = kList / kThreads;
         uint64_t w[kEach], sum = 0, unused;
 #pragma unroll
         for (int y = 0; y < kEach; ++y) {
           const int x = tid * kEach + y;
-          w[y] = x < static_cast<int>(in_bin) ? weight(r.e(key_logit(sh.list[x]))) : 0;
+          w[y] = x < in_bin ? weight(r.e(key_logit(sh.list[x]))) : 0;
           sum += w[y];
         }
         uint64_t at = before + block_before(sum, sh.warp64, unused);
@@ -484,41 +653,41 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       cluster.sync();
       cut = *cluster.map_shared_rank(&sh.cut, 0);
     } else {
-      const uint64_t from = cut;
-      cut = bisect(
-          [&](float v, int i, uint64_t at) -> uint64_t {
-            return r.bin(v) == bin && rank_key(v, i) >= (at > from ? at : from) ? weight(r.e(v)) : 0;
-          },
-          bar - before);
-      cut = cut > from ? cut : from;
+      cut = bisect([&](float v) { return weight(r.e(v)); }, static_cast<float>(bin), bin + 1.f, cut, bar - before);
     }
   }
 
   // 5: each warp a contiguous part of the CTA's range
-  auto kept = [&](int x) -> uint64_t {
-    const float v = get(x), e = r.e(v);
-    return e >= min_p && (!cut || rank_key(v, i0 + x) >= cut) ? weight(e) : 0;
+  const float cut_v = cut ? key_logit(cut) : -INFINITY;  // kept: above the cut's logit, or equal and not after its index
+  const int cut_i = cut ? key_index(cut) : 0x7fffffff;
+  auto kept_e = [&](float v, int i) {
+    const float e = r.e(v);
+    return e >= min_p && (v > cut_v || (v == cut_v && i <= cut_i)) ? e : 0.f;
   };
-  const int part = (n + kWarps - 1) / kWarps, x0 = min(n, warp * part), x1 = min(n, x0 + part);
-  uint64_t sum = 0;
-  for (int x = x0 + lane; x < x1; x += 32) sum += kept(x);
-  sum = warp_sum64(sum);
-  if (lane == 0) sh.warp_kept[warp] = sum;
-  cluster.sync();
-  uint64_t total = 0, ahead = 0;  // of the row, and of the CTAs before this one
-  for (int c = 0; c < C; ++c) {
-    const uint64_t* o = cluster.map_shared_rank(sh.warp_kept, c);
-    uint64_t t = 0;
+  const int part = (quads + kWarps - 1) / kWarps, q0 = min(quads, warp * part), q1 = min(quads, q0 + part);
+  WeightSum ws;
+#pragma unroll 2
+  for (int q = q0 + lane; q < q1; q += 32) {
+    float f[4];
+    get4(q, f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) t += o[w];
-    if (c < rank) ahead += t;
-    total += t;
+    for (int y = 0; y < 4; ++y) ws.add(kept_e(f[y], i0 + 4 * q + y));
   }
+  uint64_t sum = warp_sum64(ws.get());
+  if (lane == 0) sh.warp_kept[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += sh.warp_kept[w];
+    sh.sum[round] = sum;
+  }
+  cluster.sync();
+  sum = lane < C ? *cluster.map_shared_rank(&sh.sum[round], lane) : 0;
+  const uint64_t total = warp_sum64(sum);                // of the row
+  uint64_t ahead = warp_sum64(lane < rank ? sum : 0);    // of the CTAs before this one
   if (total == 0) {
-    if (rank == 0 && tid == 0) {
-      p.token[b] = -1;
-      if (p.prob) p.prob[b] = 0.f;
-    }
+    if (rank == 0 && tid == 0) tell(-1, 0, 0);
   } else {
     const uint64_t target = target_of(p.u[b], total);
     int found = -1;
@@ -527,22 +696,29 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       if (found < 0 && target >= ahead && target < ahead + t) found = w;
       if (found < 0) ahead += t;
     }
-    if (found >= 0) {  // this CTA, the part of warp `found`: every thread a few elements of it in order
-      const int y0 = min(n, found * part), y1 = min(n, y0 + part), each = (part + kThreads - 1) / kThreads;
+    if (found >= 0) {  // this CTA, the part of warp `found`: every thread a few fours of it in order
+      const int y0 = min(quads, found * part), y1 = min(quads, y0 + part), each = (part + kThreads - 1) / kThreads;
       const int z0 = min(y1, y0 + tid * each), z1 = min(y1, z0 + each);
-      sum = 0;
-      for (int x = z0; x < z1; ++x) sum += kept(x);
+      WeightSum mine;
+      for (int q = z0; q < z1; ++q) {
+        float f[4];
+        get4(q, f);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) mine.add(kept_e(f[y], i0 + 4 * q + y));
+      }
       uint64_t unused;
+      sum = mine.get();
       uint64_t at = ahead + block_before(sum, sh.warp64, unused);
-      for (int x = z0; x < z1; ++x) {
-        const uint64_t w = kept(x);
-        if (target >= at && target < at + w) {
-          p.token[b] = i0 + x;
-          if (p.prob)
-            p.prob[b] = static_cast<float>(__ddiv_rn(__ll2double_rn(static_cast<long long>(w)),
-                                                     __ll2double_rn(static_cast<long long>(total))));
+      if (target >= at && target < at + sum) {
+        for (int q = z0; q < z1; ++q) {
+          float f[4];
+          get4(q, f);
+          for (int y = 0; y < 4; ++y) {
+            const uint64_t w = weight(kept_e(f[y], i0 + 4 * q + y));
+            if (target >= at && target < at + w) tell(i0 + 4 * q + y, w, total);
+            at += w;
+          }
         }
-        at += w;
       }
     }
   }
@@ -579,13 +755,13 @@ int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
   int c = 1;
   while (c < most[dev] && p.V > c * 2048 && (p.B * c < ctx->num_sms || p.V / c > 24000)) c *= 2;
   p.per = (p.V + c - 1) / c;
-  const int fixed = static_cast<int>(align16(sizeof(Shared))) + 16;
-  const int room = (ctx->max_smem_optin - fixed) / 4;
-  p.cached = p.per < room ? p.per : room;
+  const int size = static_cast<int>(sizeof(typename Raw<DT>::Type)), fixed = static_cast<int>(align16(sizeof(Shared)));
+  const int room = (ctx->max_smem_optin - fixed) / size / 16 * 16, want = (p.per + 31) / 16 * 16;  // its ends' padding too
+  p.cached = want < room ? want : room;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.B) * c);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = fixed + 4 * static_cast<size_t>(p.cached);
+  cfg.dynamicSmemBytes = fixed + size * static_cast<size_t>(p.cached);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -605,7 +781,8 @@ using namespace agxc;
 extern "C" AGXC_API int agxc_sample_dev(agxc_ctx* ctx, const agxc_sample_args* a, void* stream) {
   if (!ctx || !a) return fail(AGXC_EINVAL, "sample: null argument");
   if (a->dtype < AGXC_F32 || a->dtype > AGXC_BF16) return fail(AGXC_EINVAL, "sample: logits fp32, fp16 or bf16");
-  if (a->batch < 0 || a->vocab < 1) return fail(AGXC_EINVAL, "sample: batch >= 0 and a vocabulary of at least one");
+  if (a->batch < 0 || a->batch > (1 << 26)) return fail(AGXC_EINVAL, "sample: batch 0 to 67,108,864");
+  if (a->vocab < 1 || a->vocab > (1 << 20)) return fail(AGXC_EINVAL, "sample: vocab 1 to 1,048,576");
   if (a->logits_ld < a->vocab) return fail(AGXC_EINVAL, "sample: logits_ld < vocab");
   if (!a->temperature_dev && !(a->temperature >= 0.f)) return fail(AGXC_EINVAL, "sample: temperature >= 0");
   if (a->batch == 0) return 0;
@@ -614,7 +791,7 @@ extern "C" AGXC_API int agxc_sample_dev(agxc_ctx* ctx, const agxc_sample_args* a
   p.x = a->logits_dev; p.ld = a->logits_ld; p.B = a->batch; p.V = a->vocab; p.u = a->u_dev;
   p.T = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
   p.T_a = a->temperature_dev; p.k_a = a->top_k_dev; p.p_a = a->top_p_dev; p.m_a = a->min_p_dev;
-  p.token = a->token_dev; p.prob = a->prob_dev;
+  p.token = a->token_dev; p.prob = a->prob_dev; p.err = ctx->err_dev;
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   if (a->dtype == AGXC_F32) return sample_launch<AGXC_F32>(ctx, p, s);
   if (a->dtype == AGXC_F16) return sample_launch<AGXC_F16>(ctx, p, s);
