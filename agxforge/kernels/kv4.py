@@ -32,13 +32,19 @@ import torch
 from agxforge_b200 import _native as N
 
 LOG2E = 1.4426950408889634
+_QSCALE = {hd: float(np.float32(LOG2E / math.sqrt(hd))) for hd in (64, 128)}
 DTYPES = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+
+
+# the handle of torch's current stream on a device, without a Stream object around it (1.2 us a call less)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _stream(index):
     """torch's current stream on the device; its default stream (handle 0) as cudaStreamLegacy (1), because the C ABI
     reads NULL as the context's own stream."""
-    return C.c_void_p(torch.cuda.current_stream(index).cuda_stream or 1)
+    return _raw_stream(index) or 1
 
 
 def _need(ok, text):
@@ -46,8 +52,8 @@ def _need(ok, text):
         raise ValueError(text)
 
 
-def _check(t, dtype, device, what):
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+def _check(t, dtype, index, what):
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
         raise ValueError("%s: contiguous %s on the cache's device" % (what, str(dtype)[6:]))
 
 
@@ -73,6 +79,7 @@ class KV4Cache:
         self.data, self.pages, self.kv_heads, self.head_dim, self.page_size = data, pages, kv_heads, head_dim, page_size
         self.device, self.index = data.device, data.device.index
         self._c = N.Kv4Cache(data.data_ptr(), pages, kv_heads, head_dim, page_size)
+        self._workspace = {}        # bytes that an attention call of a shape needs
 
     @classmethod
     def of(cls, data, head_dim, page_size=64):
@@ -86,11 +93,15 @@ class KV4Cache:
 
     def rows(self, slots):
         """(k, v) fp16 [tokens, kv_heads, head_dim]: the values held at `slots` (int64); zeros for a negative slot."""
-        _check(slots, torch.int64, self.device, "rows: slots")
-        k, v = torch.empty((2, slots.numel(), self.kv_heads, self.head_dim), dtype=torch.float16, device=self.device)
-        N.check(N.lib().agxc_kv4_rows_dev(N.context(self.index), C.byref(self._c), slots.data_ptr(), slots.numel(),
-                                          k.data_ptr(), v.data_ptr(), _stream(self.index)), "rows")
-        return k, v
+        idx, T = self.index, slots.numel()
+        _check(slots, torch.int64, idx, "rows: slots")
+        kv = torch.empty(2, T, self.kv_heads, self.head_dim, dtype=torch.float16, device=self.device)
+        at = kv.data_ptr()
+        rc = N.lib().agxc_kv4_rows_dev(N.context(idx), C.byref(self._c), slots.data_ptr(), T, at,
+                                       at + 2 * T * self.kv_heads * self.head_dim, _stream(idx))
+        if rc:
+            N.check(rc, "rows")
+        return kv.unbind(0)
 
 
 def append(cache, qkv, positions, slots, cos, sin, heads, bias=None, q_norm=None, k_norm=None, eps=1e-6, qscale=None,
@@ -101,44 +112,51 @@ def append(cache, qkv, positions, slots, cos, sin, heads, bias=None, q_norm=None
     [(heads + 2 kv_heads) * head_dim], q_norm and k_norm fp16 [head_dim]. qscale defaults to log2(e) / sqrt(head_dim)
     (the attention's softmax is base 2). Returns q [tokens, heads, head_dim], bf16 for bf16 rows and fp16 otherwise
     unless q_dtype says which."""
-    dev, hd, idx = cache.device, cache.head_dim, cache.index
+    hd, idx = cache.head_dim, cache.index
     width = (heads + 2 * cache.kv_heads) * hd
-    _need(heads >= 1 and heads % cache.kv_heads == 0, "append: heads a positive multiple of kv_heads")
-    _need(qkv.dim() == 2 and qkv.shape[1] == width,
-          "append: qkv is [tokens, (heads + 2 kv_heads) * head_dim] = [tokens, %d]" % width)
-    _need(qkv.dtype in DTYPES and qkv.device == dev and (qkv.stride(1) == 1 or width == 1),
-          "append: qkv fp32, fp16 or bf16 on the cache's device, its rows contiguous")
+    if heads < 1 or heads % cache.kv_heads:
+        raise ValueError("append: heads a positive multiple of kv_heads")
+    if qkv.dim() != 2 or qkv.shape[1] != width:
+        raise ValueError("append: qkv is [tokens, (heads + 2 kv_heads) * head_dim] = [tokens, %d]" % width)
     T = qkv.shape[0]
-    _check(positions, torch.int32, dev, "append: positions")
-    _check(slots, torch.int64, dev, "append: slots")
-    _need(positions.numel() == T and slots.numel() == T, "append: one position and one slot a token")
-    _check(cos, torch.float32, dev, "append: cos")
-    _check(sin, torch.float32, dev, "append: sin")
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == hd // 2 and cos.shape[0] >= 1,
-          "append: cos and sin are [n, head_dim / 2]")
+    ld, inner = qkv.stride()
+    kind = DTYPES.get(qkv.dtype)
+    if kind is None or qkv.get_device() != idx or inner != 1:
+        raise ValueError("append: qkv fp32, fp16 or bf16 on the cache's device, its rows contiguous")
+    _check(positions, torch.int32, idx, "append: positions")
+    _check(slots, torch.int64, idx, "append: slots")
+    if positions.numel() != T or slots.numel() != T:
+        raise ValueError("append: one position and one slot a token")
+    _check(cos, torch.float32, idx, "append: cos")
+    _check(sin, torch.float32, idx, "append: sin")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or cos.shape[0] < 1:
+        raise ValueError("append: cos and sin are [n, head_dim / 2]")
     if bias is not None:
-        _check(bias, torch.float16, dev, "append: bias")
+        _check(bias, torch.float16, idx, "append: bias")
         _need(bias.numel() == width, "append: bias is [(heads + 2 kv_heads) * head_dim]")
     _need((q_norm is None) == (k_norm is None), "append: q_norm and k_norm, or neither")
     if q_norm is not None:
         for g in (q_norm, k_norm):
-            _check(g, torch.float16, dev, "append: q_norm and k_norm")
+            _check(g, torch.float16, idx, "append: q_norm and k_norm")
             _need(g.numel() == hd, "append: q_norm and k_norm are [head_dim]")
     if out is None:
         if q_dtype is None:
-            q_dtype = torch.bfloat16 if qkv.dtype == torch.bfloat16 else torch.float16
-        out = torch.empty((T, heads, hd), dtype=q_dtype, device=dev)
+            q_dtype = torch.bfloat16 if kind == N.BF16 else torch.float16
+        _need(q_dtype is torch.float16 or q_dtype is torch.bfloat16, "append: q fp16 or bf16")
+        out = torch.empty(T, heads, hd, dtype=q_dtype, device=cache.device)
     else:
-        _check(out, out.dtype, dev, "append: out")
+        _need(out.dtype in (torch.float16, torch.bfloat16), "append: q fp16 or bf16")
+        _check(out, out.dtype, idx, "append: out")
         _need(out.shape == (T, heads, hd), "append: out is [tokens, heads, head_dim]")
-    _need(out.dtype in (torch.float16, torch.bfloat16), "append: q fp16 or bf16")
     if qscale is None:
-        qscale = float(np.float32(LOG2E / math.sqrt(hd)))
-    a = N.Kv4AppendArgs(cache._c, qkv.data_ptr(), qkv.stride(0) if T > 1 else width, DTYPES[qkv.dtype], T, heads,
-                        positions.data_ptr(), slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        qscale = _QSCALE[hd]
+    a = N.Kv4AppendArgs(cache._c, qkv.data_ptr(), ld if T > 1 else width, kind, T, heads, positions.data_ptr(),
+                        slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
                         None if bias is None else bias.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
                         None if k_norm is None else k_norm.data_ptr(), eps, qscale, out.data_ptr(), DTYPES[out.dtype])
-    N.check(N.lib().agxc_kv4_append_dev(N.context(idx), C.byref(a), _stream(idx)), "append")
+    rc = N.lib().agxc_kv4_append_dev(N.context(idx), C.byref(a), _stream(idx))
+    if rc:
+        N.check(rc, "append")
     return out
 
 
@@ -147,35 +165,45 @@ def attention(q, cache, page_table, lengths, out=None):
     [batch, heads, head_dim] or [batch, rows, heads, head_dim], over the cache: page_table int32 [batch, max_pages]
     (its rows may be strided), lengths int32 [batch], the tokens held with the rows' own among them. Returns out of
     q's shape and type."""
-    dev, idx = cache.device, cache.index
-    _need(q.dim() in (3, 4) and q.shape[-1] == cache.head_dim,
-          "attention: q is [batch, heads, head_dim] or [batch, rows, heads, head_dim] with head_dim %d" % cache.head_dim)
-    _need(q.dtype in (torch.float16, torch.bfloat16) and q.device == dev, "attention: q fp16 or bf16 on the cache's device")
-    B, n, H = q.shape[0], 1 if q.dim() == 3 else q.shape[1], q.shape[-2]
-    _need(H >= 1 and H % cache.kv_heads == 0, "attention: heads a positive multiple of kv_heads")
-    _check(lengths, torch.int32, dev, "attention: lengths")
-    _need(lengths.numel() == B, "attention: one length a sequence")
-    _need(page_table.dim() == 2 and page_table.shape[0] == B and page_table.dtype == torch.int32 and
-          page_table.device == dev and (page_table.stride(1) == 1 or page_table.shape[1] <= 1),
-          "attention: page_table int32 [batch, max_pages] on the cache's device, its rows contiguous")
+    hd, idx = cache.head_dim, cache.index
+    shape = q.shape
+    if len(shape) not in (3, 4) or shape[-1] != hd:
+        raise ValueError("attention: q is [batch, heads, head_dim] or [batch, rows, heads, head_dim] with head_dim %d" % hd)
+    kind = DTYPES.get(q.dtype)
+    if kind is None or kind == N.F32 or q.get_device() != idx:
+        raise ValueError("attention: q fp16 or bf16 on the cache's device")
+    B, n, H = shape[0], 1 if len(shape) == 3 else shape[1], shape[-2]
+    if H < 1 or H % cache.kv_heads:
+        raise ValueError("attention: heads a positive multiple of kv_heads")
+    _check(lengths, torch.int32, idx, "attention: lengths")
+    if lengths.numel() != B:
+        raise ValueError("attention: one length a sequence")
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype is not torch.int32 or \
+            page_table.get_device() != idx or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError("attention: page_table int32 [batch, max_pages] on the cache's device, its rows contiguous")
     if not q.is_contiguous():
         q = q.contiguous()
     if out is None:
         out = torch.empty_like(q)
     else:
-        _check(out, q.dtype, dev, "attention: out")
-        _need(out.shape == q.shape, "attention: out has q's shape")
+        _check(out, q.dtype, idx, "attention: out")
+        _need(out.shape == shape, "attention: out has q's shape")
     mp = page_table.shape[1]
-    a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), DTYPES[q.dtype], B, n, H, page_table.data_ptr(),
+    a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), kind, B, n, H, page_table.data_ptr(),
                            page_table.stride(0) if B > 1 else mp, mp, lengths.data_ptr(), None, 0)
     L, ctx = N.lib(), N.context(idx)
-    need = L.agxc_kv4_attention_workspace(ctx, C.byref(a))
-    if need < 0:
-        N.check(N.EINVAL, "attention")
+    need = cache._workspace.get((B, n, H, mp))
+    if need is None:
+        need = L.agxc_kv4_attention_workspace(ctx, C.byref(a))
+        if need < 0:
+            N.check(N.EINVAL, "attention")
+        cache._workspace[B, n, H, mp] = need
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
         a.workspace_dev, a.workspace_bytes = ws.data_ptr(), need
-    N.check(L.agxc_kv4_attention_dev(ctx, C.byref(a), _stream(idx)), "attention")
+    rc = L.agxc_kv4_attention_dev(ctx, C.byref(a), _stream(idx))
+    if rc:
+        N.check(rc, "attention")
     return out
 
 

@@ -17,14 +17,14 @@ import ctypes as C
 import torch
 
 from agxforge_b200 import _native as N
-from agxforge.kernels.kv4 import DTYPES, _need, _stream
+from agxforge.kernels.kv4 import DTYPES, _stream
 
 
-def _option(v, dtype, B, device, name):
+def _option(v, dtype, B, index, name):
     """(number, device pointer): a number for all rows, or a tensor with one a row."""
     if isinstance(v, torch.Tensor):
-        _need(v.dtype == dtype and v.device == device and v.numel() == B and v.is_contiguous(),
-              "sample: %s is a number or contiguous %s [batch] on the logits' device" % (name, str(dtype)[6:]))
+        if v.dtype is not dtype or v.get_device() != index or v.numel() != B or not v.is_contiguous():
+            raise ValueError("sample: %s is a number or contiguous %s [batch] on the logits' device" % (name, str(dtype)[6:]))
         return 0, v.data_ptr()
     return v, None
 
@@ -33,21 +33,25 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Tokens int32 [batch] and their probabilities fp32 [batch] for logits [batch, vocab] fp32, fp16 or bf16 (rows may
     be strided) and u fp32 [batch] in [0, 1). temperature, top_p and min_p: numbers or fp32 [batch]; top_k: a number or
     int32 [batch]."""
-    _need(logits.dim() == 2 and logits.dtype in DTYPES and logits.is_cuda and logits.shape[1] >= 1 and
-          (logits.stride(1) == 1 or logits.shape[1] == 1),
-          "sample: logits are [batch, vocab] fp32, fp16 or bf16 on the GPU, their rows contiguous")
+    kind, idx = DTYPES.get(logits.dtype), logits.get_device()
+    if logits.dim() != 2 or kind is None or idx < 0 or logits.shape[1] < 1 or \
+            (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("sample: logits are [batch, vocab] fp32, fp16 or bf16 on the GPU, their rows contiguous")
     B, V = logits.shape
+    if u.dtype is not torch.float32 or u.get_device() != idx or u.numel() != B or not u.is_contiguous():
+        raise ValueError("sample: u is contiguous float32 [batch] on the logits' device")
+    t, td = _option(temperature, torch.float32, B, idx, "temperature")
+    k, kd = _option(top_k, torch.int32, B, idx, "top_k")
+    p, pd = _option(top_p, torch.float32, B, idx, "top_p")
+    m, md = _option(min_p, torch.float32, B, idx, "min_p")
+    if not t >= 0:
+        raise ValueError("sample: temperature >= 0")
     dev = logits.device
-    _need(u.dtype == torch.float32 and u.device == dev and u.numel() == B and u.is_contiguous(),
-          "sample: u is contiguous float32 [batch] on the logits' device")
-    t, td = _option(temperature, torch.float32, B, dev, "temperature")
-    k, kd = _option(top_k, torch.int32, B, dev, "top_k")
-    p, pd = _option(top_p, torch.float32, B, dev, "top_p")
-    m, md = _option(min_p, torch.float32, B, dev, "min_p")
-    _need(t >= 0, "sample: temperature >= 0")
     tokens = torch.empty(B, dtype=torch.int32, device=dev)
     probs = torch.empty(B, dtype=torch.float32, device=dev)
-    a = N.SampleArgs(logits.data_ptr(), logits.stride(0) if B > 1 else V, DTYPES[logits.dtype], B, V, u.data_ptr(), t, p, m,
-                     k, td, kd, pd, md, tokens.data_ptr(), probs.data_ptr())
-    N.check(N.lib().agxc_sample_dev(N.context(dev.index), C.byref(a), _stream(dev.index)), "sample")
+    a = N.SampleArgs(logits.data_ptr(), logits.stride(0) if B > 1 else V, kind, B, V, u.data_ptr(), t, p, m, k, td, kd, pd,
+                     md, tokens.data_ptr(), probs.data_ptr())
+    rc = N.lib().agxc_sample_dev(N.context(idx), C.byref(a), _stream(idx))
+    if rc:
+        N.check(rc, "sample")
     return tokens, probs

@@ -22,13 +22,16 @@
 // share of that line, whatever the lengths are. A fifth warp copies the blocks, a bulk copy a tile (which is
 // contiguous), into three stages of shared memory, and each of four warps computes on 32 keys of a block. A piece that
 // is not a whole item leaves its maximum, sum and values in the workspace, and a second kernel joins the pieces in a
-// fixed order (no atomics: equal calls give equal bits).
-#include <cfloat>
+// fixed order (no atomics: equal calls give equal bits). Few items (a sequence or three) are split over a cluster each
+// instead, whose CTAs join their pieces in shared memory: one launch, and no second kernel to wait for.
+#include <cooperative_groups.h>
 
 #include "kv4.cuh"
 
 namespace agxc {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;       // of the warps that compute; one more warp copies
@@ -40,7 +43,7 @@ struct Kv4AttnParams {
   const void* q;
   void* out;
   int B, n, H, G, CB;                   // G = q heads a KV head, CB = column blocks an item row
-  int table_ld, max_pages, ctas;
+  int table_ld, max_pages, ctas, cluster;  // cluster = CTAs an item, 0 = the line
   const int32_t* table;
   const int32_t* lengths;
   float* part;                          // [2 ctas][columns]{max, sum}, then [2 ctas][columns][hd]
@@ -202,12 +205,38 @@ struct Smem {
   static constexpr int kRow = HD + 4;
   static constexpr int kO = kStages * kStage;
   static constexpr int kMl = kO + kWarps * kCols * kRow * 4;
-  static constexpr int kBar = kMl + kWarps * kCols * 8;
+  static constexpr int kOwn = kMl + kWarps * kCols * 8;   // {max, sum} of the CTA, for its cluster
+  static constexpr int kBar = kOwn + kCols * 8;
   static constexpr int kCame = kBar + 2 * kStages * 8;
   static constexpr int kBytes = kCame + kStages * 4;
 };
 
-template <int HD, int NT, typename T>
+// Sixteen lanes' results of one column's eight dims, {m, sum} and v each, as one: out on every lane.
+__device__ __forceinline__ void join16(float m, float sum, float* v) {
+  float mx = m;
+#pragma unroll
+  for (int x = 8; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  const float f = ex2(m - mx);
+  sum *= f;
+#pragma unroll
+  for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  const float inv = sum > 0.f ? f / sum : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] *= inv;
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
+  }
+}
+
+template <int HD, typename T>
+__device__ __forceinline__ void write8(const Kv4AttnParams& p, int b, int j, int col, int d, const float* v) {
+  T* dst = static_cast<T*>(p.out) +
+           ((static_cast<long long>(b) * p.n + col / p.G) * p.H + j * p.G + col % p.G) * HD + d;
+  *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
+}
+
+template <int HD, int NT, typename T, bool CL>
 __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
   using Tile = Kv4Tile<HD>;
@@ -232,9 +261,20 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
   pdl_wait();
   pdl_launch_dependents();
 
-  const long long quota = line_quota(p, lane);
   Place at;
-  {
+  if constexpr (CL) {
+    const int unit = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+    at.b = unit / (p.c.kvh * p.CB);
+    at.item = unit % (p.c.kvh * p.CB);
+    at.len = seq_len(p, at.b);
+    at.T = blocks_of(at.len);
+    const int per = (at.T + p.cluster - 1) / p.cluster;
+    at.t = rank * per;
+    at.rem = min(per, max(0, at.T - at.t));
+    if (threadIdx.x < NC) reinterpret_cast<float2*>(sm + Sm::kOwn)[threadIdx.x] = make_float2(kNone, 0.f);
+    __syncthreads();
+  } else {
+    const long long quota = line_quota(p, lane);
     const long long from = quota * blockIdx.x;
     long long start;
     if (quota == 0 || !line_find(p, lane, from, at.b, at.len, start)) return;  // every warp of the CTA alike
@@ -256,10 +296,10 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     unsigned uses = 0;
     int stage = 0;
     bool dead = false;
-    for (; at.rem > 0 && !dead; at.next(p)) {
-      const int tiles = (at.len + 15) >> 4, end = seen(at);
-      const int32_t* row = p.table + static_cast<long long>(at.b) * p.table_ld;
-      for (int blk = at.t; blk < end; ++blk) {
+    for (Place w = at; w.rem > 0 && !dead; w.next(p)) {
+      const int tiles = (w.len + 15) >> 4, end = seen(w);
+      const int32_t* row = p.table + static_cast<long long>(w.b) * p.table_ld;
+      for (int blk = w.t; blk < end; ++blk) {
         const int tile = blk * (kBlock / 16) + lane;
         const bool mine = lane < kBlock / 16 && tile < tiles;
         const int page = mine ? __ldg(row + tile / tiles_page) : -1;
@@ -276,7 +316,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         }
         __syncwarp();
         if (ok)
-          bulk_g2s(sm + stage * Sm::kStage + lane * Tile::kBytes, Tile::ptr(p.c, page, at.item / p.CB, tile % tiles_page),
+          bulk_g2s(sm + stage * Sm::kStage + lane * Tile::kBytes, Tile::ptr(p.c, page, w.item / p.CB, tile % tiles_page),
                    Tile::kBytes, &full[stage]);
         stage = stage + 1 == S ? 0 : stage + 1;
         ++uses;
@@ -284,8 +324,10 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     }
     // every copy lands before the CTA's memory is another's
     for (unsigned x = uses < S ? 0 : uses - S; x < uses; ++x) mbar_wait_quiet(&full[x % S], x / S & 1, p.err);
-    return;
+    if constexpr (!CL) return;
+    at.rem = 0;
   }
+  const int cl_item = at.item, cl_b = at.b;
 
   bool dead = false;                        // a wait gave up: the error word says so, and nothing more is computed
   int slot = 0, phase = 0;
@@ -597,7 +639,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
       }
     warps_sync();
     // the four warps joined; whole items are written out, pieces go to the workspace
-    const bool whole = at.t == 0 && at.end() == at.T;
+    const bool whole = !CL && at.t == 0 && at.end() == at.T;
     const int piece = 2 * blockIdx.x + (at.t == 0 ? 1 : 0);
     for (int u = threadIdx.x; u < cols * (HD / 8); u += kThreads) {
       const int col = u / (HD / 8), d = u % (HD / 8) * 8;
@@ -620,10 +662,12 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        const int i = (col0 + col) / p.G;
-        T* dst = static_cast<T*>(p.out) +
-                 ((static_cast<long long>(at.b) * p.n + i) * p.H + j * p.G + (col0 + col) % p.G) * HD + d;
-        *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
+        write8<HD, T>(p, at.b, j, col0 + col, d, v);
+      } else if (CL) {                       // this thread's own place among the first warp's results
+        float* dst = so + col * Sm::kRow + d;
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        if (d == 0) reinterpret_cast<float2*>(sm + Sm::kOwn)[col] = make_float2(mx, sum);
       } else {
         float* ml_out = p.part + (static_cast<long long>(piece) * NC + col) * 2;
         float* dst = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2 + (static_cast<long long>(piece) * NC + col) * HD + d;
@@ -632,8 +676,30 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
       }
     }
+    if constexpr (CL) break;
     warps_sync();
     at.next(p);
+  }
+  if constexpr (CL) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int rank = blockIdx.x % p.cluster, j = cl_item / p.CB, col0 = cl_item % p.CB * NC;
+    const int units = min(NC, p.n * p.G - col0) * (HD / 8);
+    for (int u0 = (rank * kWarps + warp) * 2; warp < kWarps && u0 < units; u0 += p.cluster * kWarps * 2) {
+      const int u = min(u0 + (lane >> 4), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8, x = lane & 15;
+      float2 ml = make_float2(kNone, 0.f);
+      float v[8] = {};
+      if (x < p.cluster) ml = *cluster.map_shared_rank(reinterpret_cast<float2*>(sm + Sm::kOwn) + col, x);
+      if (ml.y > 0.f) {
+        const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(so + col * Sm::kRow + d, x));
+        const float4 a = src[0], e = src[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = e.x; v[5] = e.y; v[6] = e.z; v[7] = e.w;
+      }
+      join16(ml.x, ml.y, v);
+      if (x == 0 && u0 + (lane >> 4) < units) write8<HD, T>(p, cl_b, j, col0 + col, d, v);
+    }
+    cluster.sync();                          // the neighbours' shared memory stays until all have read it
   }
 }
 
@@ -644,7 +710,7 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
   constexpr int NC = 8 * NT;
   const int lane = threadIdx.x & 31;
   const int items = p.c.kvh * p.CB, b = blockIdx.x / items, item = blockIdx.x % items;
-  pdl_wait();
+  // The lengths may be read before the first kernel is done: it let this one start after its own wait.
   const int blocks = blocks_of(seq_len(p, b));
   const int j = item / p.CB, col0 = item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
   long long c0 = 0, c1 = 0;
@@ -657,35 +723,48 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
     const long long start = before * items + static_cast<long long>(item) * blocks;
     c0 = start / quota;
     c1 = (start + blocks - 1) / quota;
-    if (c0 == c1) return;                   // one CTA had all of it
   }
-  for (int u = threadIdx.x; u < cols * (HD / 8); u += kThreads) {
-    const int col = u / (HD / 8), d = u % (HD / 8) * 8;
-    float v[8] = {};
-    if (blocks) {
-      const float* ml = p.part;
-      const float* val = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2;
-      float mx = kNone, sum = 0.f;
-      for (long long x = c0; x <= c1; ++x)
-        mx = fmaxf(mx, __ldcg(ml + ((2 * x + (x == c0)) * NC + col) * 2));
-      for (long long x = c0; x <= c1; ++x) {
-        const long long k = (2 * x + (x == c0)) * NC + col;
-        const float2 q = __ldcg(reinterpret_cast<const float2*>(ml) + k);
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d));
-        const float4 e = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d + 4));
-        const float f = ex2(q.x - mx);
-        sum = fmaf(f, q.y, sum);
-        v[0] = fmaf(f, a.x, v[0]); v[1] = fmaf(f, a.y, v[1]); v[2] = fmaf(f, a.z, v[2]); v[3] = fmaf(f, a.w, v[3]);
-        v[4] = fmaf(f, e.x, v[4]); v[5] = fmaf(f, e.y, v[5]); v[6] = fmaf(f, e.z, v[6]); v[7] = fmaf(f, e.w, v[7]);
-      }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= inv;
+  pdl_wait();
+  if (blocks && c0 == c1) return;           // one CTA had all of it
+  const float* ml = p.part;
+  const float* val = p.part + static_cast<long long>(p.ctas) * 2 * NC * 2;
+  const int units = cols * (HD / 8);
+  struct Sum {  // pieces of one column's eight dims, taken in one after another
+    float m = kNone, sum = 0.f, v[8] = {};
+    __device__ void add(const float* ml, const float* val, long long k, int d) {
+      const float2 q = __ldcg(reinterpret_cast<const float2*>(ml) + k);
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d));
+      const float4 e = __ldcg(reinterpret_cast<const float4*>(val + k * HD + d + 4));
+      const float nm = fmaxf(m, q.x), f = ex2(m - nm), g = ex2(q.x - nm);
+      m = nm;
+      sum = fmaf(f, sum, g * q.y);
+      v[0] = fmaf(f, v[0], g * a.x); v[1] = fmaf(f, v[1], g * a.y); v[2] = fmaf(f, v[2], g * a.z);
+      v[3] = fmaf(f, v[3], g * a.w); v[4] = fmaf(f, v[4], g * e.x); v[5] = fmaf(f, v[5], g * e.y);
+      v[6] = fmaf(f, v[6], g * e.z); v[7] = fmaf(f, v[7], g * e.w);
     }
-    const int i = (col0 + col) / p.G;
-    T* dst = static_cast<T*>(p.out) +
-             ((static_cast<long long>(b) * p.n + i) * p.H + j * p.G + (col0 + col) % p.G) * HD + d;
-    *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
+  };
+  if (c1 - c0 < 8) {  // few pieces: a thread a (column, eight dims)
+    for (int u = threadIdx.x; u < units; u += kThreads) {
+      const int col = u / (HD / 8), d = u % (HD / 8) * 8;
+      Sum t;
+      if (blocks) {
+#pragma unroll 4
+        for (long long x = c0; x <= c1; ++x) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
+      }
+      const float inv = t.sum > 0.f ? 1.f / t.sum : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t.v[e] *= inv;
+      write8<HD, T>(p, b, j, col0 + col, d, t.v);
+    }
+    return;
+  }
+  // many: sixteen lanes, a piece each in turn
+  for (int u0 = (threadIdx.x >> 5) * 2; u0 < units; u0 += kWarps * 2) {
+    const int u = min(u0 + (lane >> 4), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8;
+    Sum t;
+    for (long long x = c0 + (lane & 15); x <= c1; x += 16) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
+    join16(t.m, t.sum, t.v);
+    if ((lane & 15) == 0 && u0 + (lane >> 4) < units) write8<HD, T>(p, b, j, col0 + col, d, t.v);
   }
 }
 
@@ -705,11 +784,14 @@ int attn_check(const agxc_kv4_attention_args* a) {
   return 0;
 }
 
-// The launch's shape: 16 columns a block where one row's heads do not fill 8, and as many CTAs as the GPU holds at once
-// (three an SM with 8 columns, two with 16), or fewer where the longest lengths possible have fewer blocks.
+// The launch's shape: 16 columns a block where one row's heads do not fill 8. Up to an eighth as many items as the GPU
+// holds CTAs (three an SM with 8 columns, two with 16): a cluster each, of as many CTAs as fit, at most 16 or one a block
+// of the longest sequence possible. More: the line, over all CTAs that the GPU holds at once. (1 x 1,792 tokens of 8 KV
+// heads: 12.4 us as a line of 112 CTAs and its join, 7.0 as clusters; the line balances what the clusters cannot, unequal
+// lengths, where they have few CTAs each.)
 struct Shape {
-  int nt, cb, ctas;
-  int64_t bytes(int hd) const { return static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
+  int nt, cb, ctas, cluster;
+  int64_t bytes(int hd) const { return cluster ? 0 : static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
 };
 
 Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
@@ -717,10 +799,18 @@ Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   const int64_t cols = static_cast<int64_t>(a->rows) * (a->heads / a->cache.kv_heads);
   s.nt = cols > 8 ? 2 : 1;
   s.cb = static_cast<int>((cols + 8 * s.nt - 1) / (8 * s.nt));
-  const int64_t blocks = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb *
-                        ((static_cast<int64_t>(a->max_pages) * a->cache.page_size + kBlock - 1) / kBlock);
+  const int64_t items = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb;
+  const int64_t longest = (static_cast<int64_t>(a->max_pages) * a->cache.page_size + kBlock - 1) / kBlock;
   const int64_t full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
-    s.ctas = static_cast<int>(blocks < 1 ? 1 : blocks < full ? blocks : full);
+  s.cluster = 0;
+  if (items * 8 <= full || (longest <= 1 && items <= 0x7fffffff)) {
+    s.cluster = 1;
+    while (s.cluster < ctx->max_cluster && s.cluster < 16 && s.cluster < longest && items * s.cluster * 2 <= full) s.cluster *= 2;
+    s.ctas = static_cast<int>(items * s.cluster);
+    return s;
+  }
+  const int64_t blocks = items * longest;
+  s.ctas = static_cast<int>(blocks < full ? blocks : full);
   return s;
 }
 
@@ -730,11 +820,33 @@ int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
   static bool allowed[64] = {};
   int dev = 0;
   AGXC_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && !allowed[dev]) {
-    AGXC_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (dev >= 64) return fail(AGXC_EINVAL, "kv4_attention: device index below 64");
+  auto* line = kv4_attn_kernel<HD, NT, T, false>;
+  auto* clusters = kv4_attn_kernel<HD, NT, T, true>;
+  if (!allowed[dev]) {
+    AGXC_CUDA(cudaFuncSetAttribute(line, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    AGXC_CUDA(cudaFuncSetAttribute(clusters, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    AGXC_CUDA(cudaFuncSetAttribute(clusters, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     allowed[dev] = true;
   }
-  if (int rc = launch_ex(kv4_attn_kernel<HD, NT, T>, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
+  if (p.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.ctas);
+    cfg.blockDim = dim3(kThreads + 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    AGXC_CUDA(cudaLaunchKernelEx(&cfg, clusters, p));
+    return 0;
+  }
+  if (int rc = launch_ex(line, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
   return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(kThreads), 0, s,
                    1, p);
 }
@@ -766,13 +878,13 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
   if (reinterpret_cast<uintptr_t>(a->q_dev) % 16 || reinterpret_cast<uintptr_t>(a->out_dev) % 16)
     return fail(AGXC_EINVAL, "kv4_attention: q and out must be 16-byte aligned");
   const Shape sh = attn_shape(ctx, a);
-  if (a->workspace_bytes < sh.bytes(a->cache.head_dim) || !a->workspace_dev ||
-      reinterpret_cast<uintptr_t>(a->workspace_dev) % 16)
+  const int64_t need = sh.bytes(a->cache.head_dim);
+  if (need && (a->workspace_bytes < need || !a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16))
     return fail(AGXC_EINVAL, "kv4_attention: a 16-byte aligned workspace of agxc_kv4_attention_workspace bytes");
   Kv4AttnParams p;
   p.c = kv4_of(a->cache);
   p.q = a->q_dev; p.out = a->out_dev; p.B = a->batch; p.n = a->rows; p.H = a->heads;
-  p.G = a->heads / a->cache.kv_heads; p.CB = sh.cb; p.ctas = sh.ctas;
+  p.G = a->heads / a->cache.kv_heads; p.CB = sh.cb; p.ctas = sh.ctas; p.cluster = sh.cluster;
   p.table_ld = a->table_ld; p.max_pages = a->max_pages; p.table = a->page_table_dev; p.lengths = a->lengths_dev;
   p.part = static_cast<float*>(a->workspace_dev); p.err = ctx->err_dev;
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
