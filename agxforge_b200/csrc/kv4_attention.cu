@@ -138,7 +138,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -150,14 +150,17 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
 
-// D = A B, m16n8k16
-__device__ __forceinline__ void mma_16816_zero(float& d0, float& d1, float& d2, float& d3, uint32_t a0, uint32_t a1,
-                                               uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%10,%10,%10,%10};\n"
-      : "=f"(d0), "=f"(d1), "=f"(d2), "=f"(d3)
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// D = A B + D and D = A B, m16n8k16 (not volatile: the compiler may order them among each other's operands)
+__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t* b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         const uint32_t* b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 
 __device__ __forceinline__ void unpack8(const uint4& u, float* f, const __half*) {
@@ -455,8 +458,8 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float* x = d[nt][g];
-                if (w + up == 0) mma_16816_zero(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][0][0], qf[nt][g][0][1]);
-                else mma_16816(x[0], x[1], x[2], x[3], f0, f1, f2, f3, qf[nt][g][w][2 * up], qf[nt][g][w][2 * up + 1]);
+                if (w + up == 0) mma_zero(x, f0, f1, f2, f3, qf[nt][g][0]);
+                else mma(x, f0, f1, f2, f3, qf[nt][g][w] + 2 * up);
               }
             }
 #pragma unroll
@@ -589,20 +592,14 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float* x = o[nt][g][k];
-              mma_16816(x[0], x[1], x[2], x[3], a[k] & 0x000f000fu, a[k] & 0x00f000f0u, b[k] & 0x000f000fu,
-                        b[k] & 0x00f000f0u, pf[nt][g][0], pf[nt][g][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+              mma(o[nt][g][k], a[k] & 0x000f000fu, a[k] & 0x00f000f0u, b[k] & 0x000f000fu, b[k] & 0x00f000f0u, pf[nt][g]);
           // -8 as the fields have it: 8 and 16 x 8 steps of 2^-24 below zero
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float* x = o[nt][g][k];
-              mma_16816(x[0], x[1], x[2], x[3], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][g][0],
-                        pf[nt][g][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+              mma(o[nt][g][k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][g]);
         }
       }
       }
