@@ -12,8 +12,7 @@
 // q is scaled by a power of two a column and the fields' 2^-24 is undone in fp32 (exact). P = p s / sref is rounded to
 // fp16 (11 bits; the only rounding of the pass): sref is the running power of two above the group's scales and the
 // reference m sits 8 below the running maximum, so P stays in fp16's normal range down to 2^-22 of the largest weight.
-// The values' codes are taken about 8 (a second MMA with the constant -8 in A follows each) and their bias as b + 8 s, so
-// that P's rounding counts by a value's distance from its group's middle and the sums over thousands of keys stay
+// The values' codes are taken about 8 (one subtraction of fp16 subnormals for two) and their bias as b + 8 s, so that P's rounding counts by a value's distance from its group's middle and the sums over thousands of keys stay
 // small beside what the tensor core's accumulation drops (codes of one sign: 3.6e-4 off at 8,192 keys, 2-norm; about 8:
 // 2.8e-4, of which the output's own fp16 rounding is 2.1e-4). m and sref move only when a score passes m + 12 or a
 // scale passes 8 sref (one vote for 32 keys), which rescales the accumulators.
@@ -34,8 +33,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;       // of the warps that compute; one more warp copies
-constexpr int kBlock = 32 * kWarps;         // keys a block
+constexpr int kThreads = 32 * kWarps;   // of the warps that compute; one more warp copies
+constexpr int kBlock = 32 * kWarps;     // keys a block
 constexpr float kNone = -1e30f;         // the maximum that stands for no key
 
 struct Kv4AttnParams {
@@ -43,7 +42,8 @@ struct Kv4AttnParams {
   const void* q;
   void* out;
   int B, n, H, G, CB;                   // G = q heads a KV head, CB = column blocks an item row
-  int table_ld, max_pages, ctas, cluster;  // cluster = CTAs an item, 0 = the line
+  int table_ld, max_pages;
+  int ctas, cluster;                    // cluster = CTAs an item, 0 = the line
   const int32_t* table;
   const int32_t* lengths;
   float* part;                          // [2 ctas][columns]{max, sum}, then [2 ctas][columns][hd]
@@ -85,6 +85,11 @@ struct Place {
   }
 };
 
+// a / b for 0 <= a, 0 < b, in 32 bits where that does
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
 // Blocks a CTA: the line's length over the CTAs. Every warp computes it for itself.
 __device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane) {
   long long sum = 0;
@@ -92,7 +97,7 @@ __device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   sum *= p.c.kvh * p.CB;
-  return (sum + p.ctas - 1) / p.ctas;
+  return quotient(sum + p.ctas - 1, p.ctas);
 }
 
 // The sequence that holds position `at` of the line, and where its items start.
@@ -149,6 +154,13 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
+
+// code - 8 of the even (hi = 0) or 16 (code - 8) of the odd nibble in the low byte of each half of x, times 2^-24 (an
+// exact difference of fp16 subnormals)
+__device__ __forceinline__ uint32_t about8(uint32_t x, int hi) {
+  const __half2 d = __hsub2(as_half2(x & (hi ? 0x00f000f0u : 0x000f000fu)), as_half2(hi ? 0x00800080u : 0x00080008u));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
 
 // D = A B + D and D = A B, m16n8k16 (not volatile: the compiler may order them among each other's operands)
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t* b) {
@@ -283,8 +295,8 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     if (quota == 0 || !line_find(p, lane, from, at.b, at.len, start)) return;  // every warp of the CTA alike
     at.T = blocks_of(at.len);
     const long long off = from - start;
-    at.item = static_cast<int>(off / at.T);
-    at.t = static_cast<int>(off % at.T);
+    at.item = static_cast<int>(quotient(off, at.T));
+    at.t = static_cast<int>(off - static_cast<long long>(at.item) * at.T);
     at.rem = quota;
   }
   // where the blocks end that some column of the item's column block sees
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     least = max(0, at.len - p.n + col0 / p.G + 1);
     most = max(0, at.len - p.n + (col0 + cols - 1) / p.G + 1);
 
-    float o[NT][GR][4][4], m[NT][2], l[NT][2], bt[NT][GR][2], sref[GR], isref[GR], big[GR];
+    float o[NT][GR][4][4], m[NT][2], l[NT][2], bt[NT][GR][2], sref[GR], isref[GR];
 #pragma unroll
     for (int g = 0; g < GR; ++g) sref[g] = 5.9604645e-8f, isref[g] = 16777216.f;
 #pragma unroll
@@ -425,7 +437,6 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
       if (mask != 0u) {
       float y[2][NT][4];                     // log2 of the weights of (key r, columns 2c, 2c + 1), (key r + 8, the same)
       uint32_t ve[2][2][GR];                 // V's {scale, bias} of keys r, r + 8
-      bool move = fresh;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint8_t* tl = st + h * Tile::kBytes;
@@ -496,17 +507,35 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
             }
           }
       }
+      // Has a weight or a scale outgrown its reference? The weights' sums of this lane's keys tell of the first (over
+      // 4,096 where one passes 2^12), each lane looks at the scales of one key for the second.
+      float pw[2][NT][4], ps[NT][2];
+      auto weigh = [&]() {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        move |= fmaxf(fmaxf(fmaxf(y[0][nt][0], y[0][nt][1]), fmaxf(y[0][nt][2], y[0][nt][3])),
-                      fmaxf(fmaxf(y[1][nt][0], y[1][nt][1]), fmaxf(y[1][nt][2], y[1][nt][3]))) > 12.f;
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {  // the low halves of the entries: V's scales
-        const __half2 a = __hmax2(__habs2(as_half2(ve[0][0][g])), __habs2(as_half2(ve[0][1][g])));
-        const __half2 b = __hmax2(__habs2(as_half2(ve[1][0][g])), __habs2(as_half2(ve[1][1][g])));
-        big[g] = __low2float(__hmax2(a, b));
-        move |= big[g] > 8.f * sref[g];
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) pw[h][nt][x] = ex2(y[h][nt][x]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            ps[nt][e] = (pw[0][nt][e] + pw[0][nt][2 + e]) + (pw[1][nt][e] + pw[1][nt][2 + e]);
+        }
+      };
+      weigh();
+      float big[GR];
+      {
+        const uint8_t* en = st + (lane >> 4) * Tile::kBytes + Tile::kSb + (lane & 15) * Tile::kEntry + 4 * GR;
+        const bool in = key0 + lane < most && (mask >> (lane >> 4) & 1u);
+#pragma unroll
+        for (int g = 0; g < GR; ++g)
+          big[g] = in ? fabsf(__half2float(*reinterpret_cast<const __half*>(en + 4 * g))) : 0.f;
       }
+      bool move = fresh;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) move |= fmaxf(ps[nt][0], ps[nt][1]) > 4096.f;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) move |= big[g] > 8.f * sref[g];
       if (__any_sync(0xffffffffu, move)) {
         float fg[GR];
 #pragma unroll
@@ -543,8 +572,14 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
               }
             }
           }
+        weigh();
       }
       fresh = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt][0] += ps[nt][0];
+        l[nt][1] += ps[nt][1];
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // weights: P operands, the sum, and the bias term
@@ -560,9 +595,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float p0 = ex2(y[h][nt][2 * i]), p1 = ex2(y[h][nt][2 * i + 1]);
-            l[nt][0] += p0;
-            l[nt][1] += p1;
+            const float p0 = pw[h][nt][2 * i], p1 = pw[h][nt][2 * i + 1];
 #pragma unroll
             for (int g = 0; g < GR; ++g) {
               bt[nt][g][0] = fmaf(p0, b8[g], bt[nt][g][0]);
@@ -590,16 +623,11 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
           const uint32_t ya = prmt(vw[0][g], vw[1][g], 0x7632u), yb = prmt(vw[2][g], vw[3][g], 0x7632u);
           const uint32_t a[4] = {xa, xa >> 8, ya, ya >> 8}, b[4] = {xb, xb >> 8, yb, yb >> 8};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a0 = about8(a[k], 0), a1 = about8(a[k], 1), a2 = about8(b[k], 0), a3 = about8(b[k], 1);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma(o[nt][g][k], a[k] & 0x000f000fu, a[k] & 0x00f000f0u, b[k] & 0x000f000fu, b[k] & 0x00f000f0u, pf[nt][g]);
-          // -8 as the fields have it: 8 and 16 x 8 steps of 2^-24 below zero
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma(o[nt][g][k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][g]);
+            for (int nt = 0; nt < NT; ++nt) mma(o[nt][g][k], a0, a1, a2, a3, pf[nt][g]);
+          }
         }
       }
       }
@@ -701,13 +729,16 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
 }
 
 // One CTA an item: joins the pieces that the CTAs of kv4_attn_kernel left of it, in their order; writes zeros for a
-// sequence of no tokens.
+// sequence of no tokens. Its few threads of 64 registers fit on an SM beside the first kernel's CTAs, so that it has
+// found its pieces when they end.
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
-  constexpr int NC = 8 * NT;
+__global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int NC = 8 * NT, kJoin = 64 * NT;
   const int lane = threadIdx.x & 31;
   const int items = p.c.kvh * p.CB, b = blockIdx.x / items, item = blockIdx.x % items;
-  // The lengths may be read before the first kernel is done: it let this one start after its own wait.
+  // The lengths may be read before the first kernel is done: it let this one start after its own wait. What follows in
+  // the stream may start to start: it waits for this kernel's end.
+  pdl_launch_dependents();
   const int blocks = blocks_of(seq_len(p, b));
   const int j = item / p.CB, col0 = item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
   long long c0 = 0, c1 = 0;
@@ -718,8 +749,8 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) before += __shfl_xor_sync(0xffffffffu, before, m);
     const long long start = before * items + static_cast<long long>(item) * blocks;
-    c0 = start / quota;
-    c1 = (start + blocks - 1) / quota;
+    c0 = quotient(start, quota);
+    c1 = quotient(start + blocks - 1, quota);
   }
   pdl_wait();
   if (blocks && c0 == c1) return;           // one CTA had all of it
@@ -741,7 +772,7 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
     }
   };
   if (c1 - c0 < 8) {  // few pieces: a thread a (column, eight dims)
-    for (int u = threadIdx.x; u < units; u += kThreads) {
+    for (int u = threadIdx.x; u < units; u += kJoin) {
       const int col = u / (HD / 8), d = u % (HD / 8) * 8;
       Sum t;
       if (blocks) {
@@ -756,7 +787,7 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const __grid_constan
     return;
   }
   // many: sixteen lanes, a piece each in turn
-  for (int u0 = (threadIdx.x >> 5) * 2; u0 < units; u0 += kWarps * 2) {
+  for (int u0 = (threadIdx.x >> 5) * 2; u0 < units; u0 += kJoin / 32 * 2) {
     const int u = min(u0 + (lane >> 4), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8;
     Sum t;
     for (long long x = c0 + (lane & 15); x <= c1; x += 16) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
@@ -797,8 +828,8 @@ Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   s.nt = cols > 8 ? 2 : 1;
   s.cb = static_cast<int>((cols + 8 * s.nt - 1) / (8 * s.nt));
   const int64_t items = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb;
-  const int64_t longest = (static_cast<int64_t>(a->max_pages) * a->cache.page_size + kBlock - 1) / kBlock;
-  const int64_t full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
+  const int64_t most = static_cast<int64_t>(a->max_pages) * a->cache.page_size;
+  const int64_t longest = (most + kBlock - 1) / kBlock, full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
   s.cluster = 0;
   if (items * 8 <= full || (longest <= 1 && items <= 0x7fffffff)) {
     s.cluster = 1;
@@ -811,22 +842,20 @@ Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   return s;
 }
 
-template <int HD, int NT, typename T>
+template <int HD, int NT, typename T, bool CL>
 int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
   constexpr int smem = Smem<HD, NT>::kBytes;
   static bool allowed[64] = {};
   int dev = 0;
   AGXC_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return fail(AGXC_EINVAL, "kv4_attention: device index below 64");
-  auto* line = kv4_attn_kernel<HD, NT, T, false>;
-  auto* clusters = kv4_attn_kernel<HD, NT, T, true>;
+  auto* kernel = kv4_attn_kernel<HD, NT, T, CL>;
   if (!allowed[dev]) {
-    AGXC_CUDA(cudaFuncSetAttribute(line, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    AGXC_CUDA(cudaFuncSetAttribute(clusters, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    AGXC_CUDA(cudaFuncSetAttribute(clusters, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (CL) AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     allowed[dev] = true;
   }
-  if (p.cluster) {
+  if (CL) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.ctas);
     cfg.blockDim = dim3(kThreads + 32);
@@ -840,17 +869,18 @@ int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    AGXC_CUDA(cudaLaunchKernelEx(&cfg, clusters, p));
+    AGXC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return 0;
   }
-  if (int rc = launch_ex(line, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
-  return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(kThreads), 0, s,
-                   1, p);
+  if (int rc = launch_ex(kernel, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
+  return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(64 * NT), 0, s, 1,
+                   p);
 }
 
 template <int HD, typename T>
-int attn_launch_nt(const Kv4AttnParams& p, int nt, cudaStream_t s) {
-  return nt == 1 ? attn_launch<HD, 1, T>(p, s) : attn_launch<HD, 2, T>(p, s);
+int attn_launch_shape(const Kv4AttnParams& p, const Shape& sh, cudaStream_t s) {
+  if (sh.cluster) return sh.nt == 1 ? attn_launch<HD, 1, T, true>(p, s) : attn_launch<HD, 2, T, true>(p, s);
+  return sh.nt == 1 ? attn_launch<HD, 1, T, false>(p, s) : attn_launch<HD, 2, T, false>(p, s);
 }
 
 }  // namespace
@@ -887,8 +917,8 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const bool bf16 = a->dtype == AGXC_BF16;
   if (a->cache.head_dim == 128)
-    return bf16 ? attn_launch_nt<128, __nv_bfloat16>(p, sh.nt, s) : attn_launch_nt<128, __half>(p, sh.nt, s);
-  return bf16 ? attn_launch_nt<64, __nv_bfloat16>(p, sh.nt, s) : attn_launch_nt<64, __half>(p, sh.nt, s);
+    return bf16 ? attn_launch_shape<128, __nv_bfloat16>(p, sh, s) : attn_launch_shape<128, __half>(p, sh, s);
+  return bf16 ? attn_launch_shape<64, __nv_bfloat16>(p, sh, s) : attn_launch_shape<64, __half>(p, sh, s);
 }
 
 }  // extern "C"
