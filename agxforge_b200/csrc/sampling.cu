@@ -8,12 +8,13 @@
 // A cluster of CTAs takes a row: each CTA reads its range of the vocabulary once into shared memory (what does not fit
 // is read again from global memory), and everything after that happens there and in its neighbours' shared memory.
 //   1  the maximum (its first index is a greedy row's token) and the least finite logit
-//   2  top-k: counts in 1,024 bins, equal steps of the logit down to weight zero or the least logit; the bin that holds
-//      rank k. Up to 2,048 elements in that bin and above go to one CTA as a list; it sorts them and finishes the row
+//   2  top-k: counts in 1,024 bins, equal steps of the logit down to weight zero or the least logit; the first CTA adds
+//      the cluster's bins up and finds the one that holds rank k. Up to 2,048 elements in that bin and above are listed,
+//      each CTA its own, and the first CTA collects them and finishes the row
 //   3  top-p: the bins' exact weights (64 bits as two 32-bit shared-memory adds, the second with the first's carry, rarely
 //      needed); the bin that holds the bar
-//   4  where a bin holds a cut, only that bin is listed and sorted, to find the key it falls on; a bin that is more than
-//      a list (thousands of equal logits) is cut bit by bit instead
+//   4  where a bin holds a cut, only that bin is listed. The key the cut falls on: 1,024 finer bins, then a comparison of
+//      the few elements of one of them. A bin that is more than a list (thousands of equal logits) is cut bit by bit
 //   5  the kept weights' total and the token, in index order: the warp, then the element, that the target falls on
 #include <cooperative_groups.h>
 
@@ -46,7 +47,7 @@ struct SampleParams {
 };
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 1024, kList = 2048, kMaxCluster = 16;
+constexpr int kFew = kThreads / 4, kBins = 1024, kList = 2048, kMaxCluster = 16;
 
 constexpr int kCopies = 4;  // pieces that a CTA's range is copied in: the first is looked at while the last are on their way
 
@@ -118,17 +119,26 @@ struct Shared {
   float2 best;  // {largest, least}
   uint64_t sum[2];
   uint64_t copied[kCopies];
-  int n_list, bin, first;
+  int n_list, n_few, bin, first;
   uint64_t before, total, cut;
+  uint64_t said[3];  // what the first CTA found
   uint64_t warp64[kWarps];
   uint64_t warp_kept[kWarps];
   alignas(16) uint32_t count[kBins];
   alignas(16) uint32_t lo[kBins];
   alignas(16) uint32_t hi[kBins];
+  uint64_t few[kFew];
   uint64_t list[kList];
 };
 
 __device__ __forceinline__ int bin_of(float place) { return __float_as_int(__fadd_rz(place, 8388608.f)) - 0x4B000000; }
+
+// one exact 64-bit sum among many in shared memory
+__device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, int at, uint64_t w) {
+  const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&lo[at], l);
+  const uint32_t h = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
+  if (h) atomicAdd(&hi[at], h);
+}
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -358,35 +368,118 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     round ^= 1;
     return t;
   };
-  // elements at places from `lo` to below `hi` whose keys reach `from`, as keys, into the first CTA's list; returns how
-  // many there are (the list holds the first kList of them)
+  // What the first CTA found, on every thread of the cluster. (It is past every reading of what it found before.)
+  auto learn = [&](uint64_t* v) {
+    cluster.sync();
+    const uint64_t o = lane < 3 ? *cluster.map_shared_rank(&sh.said[lane], 0) : 0;
+#pragma unroll
+    for (int x = 0; x < 3; ++x) v[x] = __shfl_sync(0xffffffffu, o, x);
+  };
+  // Lists the elements at places from `lo` to below `hi` whose keys reach `from`; returns their number over the cluster,
+  // all of them in the first CTA's list where they fit, to that CTA.
   auto gather = [&](float lo, float hi, uint64_t from) {
-    uint64_t* list = cluster.map_shared_rank(sh.list, 0);
-    int* count = cluster.map_shared_rank(&sh.n_list, 0);
-    for (int q0 = warp * 32; q0 < quads; q0 += kThreads) {
-      const int q = q0 + lane;
+    __syncthreads();
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    for (int q = tid; q < quads; q += kThreads) {
       float f[4];
-      bool in[4], any = false;
-      if (q < quads) get4(q, f);
+      get4(q, f);
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const float at = q < quads ? r.place(f[y]) : -1.f;
-        in[y] = at >= lo && at < hi && f[y] > -INFINITY && (!from || rank_key(f[y], i0 + 4 * q + y) >= from);
-        any |= in[y];
-      }
-      if (!__any_sync(0xffffffffu, any)) continue;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const unsigned some = __ballot_sync(0xffffffffu, in[y]);
-        if (!some) continue;
-        int at = 0;
-        if (lane == 0) at = atomicAdd(count, __popc(some));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(some & ((1u << lane) - 1));
-        if (in[y] && at < kList) list[at] = rank_key(f[y], i0 + 4 * q + y);
+        const float at = r.place(f[y]);
+        if (!(at >= lo && at < hi && f[y] > -INFINITY)) continue;
+        const uint64_t key = rank_key(f[y], i0 + 4 * q + y);
+        if (key < from) continue;
+        const int x = atomicAdd(&sh.n_list, 1);
+        if (x < kList) sh.list[x] = key;
       }
     }
     cluster.sync();
-    return *cluster.map_shared_rank(&sh.n_list, 0);
+    int len = 0;
+    if (rank == 0) {  // a warp for each CTA's list, behind this one's own
+      if (lane == 0) sh.warp64[warp] = warp < C ? *cluster.map_shared_rank(&sh.n_list, warp) : 0;
+      __syncthreads();
+      int at = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) at = len;
+        len += static_cast<int>(min(sh.warp64[w], static_cast<uint64_t>(kList + 1)));
+      }
+      if (warp > 0 && warp < C) {
+        const uint64_t* other = cluster.map_shared_rank(sh.list, warp);
+        const int m = static_cast<int>(sh.warp64[warp]);
+        for (int x = lane; x < m && at + x < kList; x += 32) sh.list[at + x] = other[x];
+      }
+      __syncthreads();
+    }
+    return len;
+  };
+  // In the first CTA: the key among the list's first `len`, all at places from `lo` to below `hi`, from which up those
+  // that reach `from` sum to `need`, by number or by weight.
+  auto cut_list = [&](int len, float lo, float hi, uint64_t from, uint64_t need, bool by_weight) {
+    const float scale = kBins / (hi - lo);
+    auto sub = [&](uint64_t key) {
+      return min(kBins - 1, max(0, __float2int_rz((r.place(key_logit(key)) - lo) * scale)));
+    };
+    auto value = [&](uint64_t key) -> uint64_t { return by_weight ? weight(r.e(key_logit(key))) : 1; };
+    __syncthreads();
+    sh.lo[tid] = sh.hi[tid] = sh.lo[tid + kThreads] = sh.hi[tid + kThreads] = 0;
+    if (tid == 0) sh.n_few = 0;
+    __syncthreads();
+    for (int x = tid; x < len; x += kThreads)
+      if (sh.list[x] >= from) add64(sh.lo, sh.hi, sub(sh.list[x]), value(sh.list[x]));
+    __syncthreads();
+    uint64_t a[2], unused;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) a[y] = static_cast<uint64_t>(sh.hi[2 * tid + y]) << 32 | sh.lo[2 * tid + y];
+    uint64_t at = block_before(a[0] + a[1], sh.warp64, unused);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      if (at < need && at + a[y] >= need) {
+        sh.bin = 2 * tid + y;
+        sh.before = at;
+      }
+      at += a[y];
+    }
+    __syncthreads();
+    const int bin = sh.bin;
+    at = sh.before;
+    for (int x = tid; x < len; x += kThreads)
+      if (sh.list[x] >= from && sub(sh.list[x]) == bin) {
+        const int z = atomicAdd(&sh.n_few, 1);
+        if (z < kFew) sh.few[z] = sh.list[x];
+      }
+    __syncthreads();
+    const int m = sh.n_few;
+    if (m <= kFew) {  // four threads an element
+      const int x = tid >> 2;
+      const uint64_t key = x < m ? sh.few[x] : 0;
+      uint64_t ahead = 0;
+      for (int y = tid & 3; y < m; y += 4)
+        if (sh.few[y] > key) ahead += value(sh.few[y]);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
+      at += ahead;
+      if (x < m && at < need && at + value(key) >= need) sh.cut = key;
+    } else {  // many equal logits: sorted
+      sort_list(sh.list, len);
+      constexpr int kEach = kList / kThreads;
+      uint64_t w[kEach], sum = 0;
+#pragma unroll
+      for (int y = 0; y < kEach; ++y) {
+        const int x = tid * kEach + y;
+        w[y] = x < len && sh.list[x] >= from ? value(sh.list[x]) : 0;
+        sum += w[y];
+      }
+      at = block_before(sum, sh.warp64, unused);
+#pragma unroll
+      for (int y = 0; y < kEach; ++y) {
+        if (at < need && at + w[y] >= need) sh.cut = sh.list[tid * kEach + y];
+        at += w[y];
+      }
+    }
+    __syncthreads();
+    return sh.cut;
   };
   auto tell = [&](int token, uint64_t w, uint64_t total) {
     p.token[b] = token;
@@ -394,9 +487,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       p.prob[b] = total ? static_cast<float>(__ddiv_rn(__ll2double_rn(static_cast<long long>(w)),
                                                        __ll2double_rn(static_cast<long long>(total)))) : 0.f;
   };
-  // The first CTA has every candidate in its list: cut, draw, done. Up to 128 candidates are ranked by comparing each
-  // with all (four threads a candidate); more are sorted, and the token is found by two histograms over the index.
-  auto finish_list = [&](int len, int keep) {
+  // The first CTA has every candidate in its list, at places below `hi`: cut, draw, done. Up to 128 candidates are ranked
+  // by comparing each with all (four threads a candidate); for more, cuts as above and two histograms over the index.
+  auto finish_list = [&](int len, float hi, int keep) {
     if (rank == 0 && len <= kThreads / 4) {
       const int x = tid >> 2;
       const uint64_t key = x < len ? sh.list[x] : 0;
@@ -438,44 +531,39 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if ((tid & 3) == 0 && target >= before && target < before + w) tell(key_index(key), w, total);
       }
     } else if (rank == 0) {
-      sort_list(sh.list, len);
-      len = min(len, keep);
-      constexpr int kEach = kList / kThreads;
-      uint64_t w[kEach], sum = 0, total, below;
-      float e[kEach];
-#pragma unroll
-      for (int y = 0; y < kEach; ++y) {
-        const int x = tid * kEach + y;
-        e[y] = x < len ? r.e(key_logit(sh.list[x])) : 0.f;
-        w[y] = x < len ? weight(e[y]) : 0;
-        sum += w[y];
+      uint64_t from = len > keep ? cut_list(len, 0.f, hi, 0, keep, false) : 0;
+      if (use_p) {
+        uint64_t sum = 0;
+        for (int x = tid; x < len; x += kThreads)
+          if (sh.list[x] >= from) sum += weight(r.e(key_logit(sh.list[x])));
+        sum = block_sum(sum, sh.warp64);
+        from = cut_list(len, 0.f, hi, from, top_p_bar(top_p, sum), true);
       }
-      below = block_before(sum, sh.warp64, total);
-      const uint64_t bar = use_p ? top_p_bar(top_p, total) : ~0ull;
-      sum = 0;
+      constexpr int kEach = kList / kThreads;
+      uint64_t w[kEach], sum = 0, total;
 #pragma unroll
       for (int y = 0; y < kEach; ++y) {
-        const uint64_t before = below;
-        below += w[y];
-        if (before >= bar || !(e[y] >= min_p)) w[y] = 0;
+        const int x = tid + y * kThreads;
+        const float e = x < len && sh.list[x] >= from ? r.e(key_logit(sh.list[x])) : 0.f;
+        w[y] = e >= min_p ? weight(e) : 0;
         sum += w[y];
       }
       total = block_sum(sum, sh.warp64);
       if (total == 0) {
         if (tid == 0) tell(-1, 0, 0);
       } else {
-        // the weights over the index in 1,024 steps, then over the indices of the step that the target falls in
-        uint64_t left = target_of(p.u[b], total);
-        int from = 0, each = (p.V + kBins - 1) / kBins;
-        uint64_t w_at = 0;
-        for (int level = 0; level < 2; ++level) {
+        // the weights over the index in up to 1,024 steps, then over the indices of the step that the target falls in
+        uint64_t left = target_of(p.u[b], total), w_at = 0;
+        const int shift = max(0, 22 - __clz(p.V - 1));  // an index has at most 20 bits
+        int at_index = 0;
+        for (int level = 0; level < (shift ? 2 : 1); ++level) {
+          sh.lo[tid] = sh.hi[tid] = sh.lo[tid + kThreads] = sh.hi[tid + kThreads] = 0;
+          __syncthreads();
 #pragma unroll
           for (int y = 0; y < kEach; ++y) {
-            const int at = w[y] ? (key_index(sh.list[tid * kEach + y]) - from) / each : -1;
-            if (at < 0 || at >= kBins) continue;
-            const uint32_t l = static_cast<uint32_t>(w[y]), old = atomicAdd(&sh.lo[at], l);
-            const uint32_t h = static_cast<uint32_t>(w[y] >> 32) + (old + l < old ? 1u : 0u);
-            if (h) atomicAdd(&sh.hi[at], h);
+            const int x = tid + y * kThreads, index = w[y] ? key_index(sh.list[x]) : 0;
+            if (w[y] && level == 1 && (index >> shift) != at_index) w[y] = 0;
+            if (w[y]) add64(sh.lo, sh.hi, level ? index & ((1 << shift) - 1) : index >> shift, w[y]);
           }
           __syncthreads();
           uint64_t a[2], unused;
@@ -484,7 +572,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           uint64_t at = block_before(a[0] + a[1], sh.warp64, unused);
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            sh.lo[2 * tid + y] = sh.hi[2 * tid + y] = 0;
             if (left >= at && left < at + a[y]) {
               sh.bin = 2 * tid + y;
               sh.before = at;
@@ -493,20 +580,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             at += a[y];
           }
           __syncthreads();
-          from += sh.bin * each;
+          at_index = level ? at_index << shift | sh.bin : sh.bin;
           left -= sh.before;
           w_at = sh.total;
-          if (level == 0) {
-            // what is outside the step counts no more
-#pragma unroll
-            for (int y = 0; y < kEach; ++y)
-              if (w[y] && (key_index(sh.list[tid * kEach + y]) < from || key_index(sh.list[tid * kEach + y]) >= from + each))
-                w[y] = 0;
-            each = 1;
-          }
           __syncthreads();
         }
-        if (tid == 0) tell(from, w_at, total);
+        if (tid == 0) tell(at_index, w_at, total);
       }
     }
     cluster.sync();
@@ -543,118 +622,111 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     }
     cluster.sync();
-    uint32_t c2[2] = {};
+    if (rank == 0) {
+      uint32_t c2[2] = {};
 #pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c)
-      if (c < C) {
-        const uint2 o = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, c) + 2 * tid);
-        c2[0] += o.x;
-        c2[1] += o.y;
-      }
-    uint64_t all;
-    uint64_t below = block_before(static_cast<uint64_t>(c2[0]) + c2[1], sh.warp64, all);
-    if (all <= static_cast<uint64_t>(k_in) && all <= kList && !use_p) {
-      // every element that weighs anything is kept: nothing to cut
-    } else {
-      if (tid == 0) sh.bin = -1;
-      __syncthreads();
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < C) {
+          const uint2 o = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, c) + 2 * tid);
+          c2[0] += o.x;
+          c2[1] += o.y;
+        }
+      uint64_t all;
+      uint64_t below = block_before(static_cast<uint64_t>(c2[0]) + c2[1], sh.warp64, all);
+      if (all < static_cast<uint64_t>(k_in) && tid == 0) sh.said[0] = kBins, sh.said[1] = 0, sh.said[2] = all;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         if (below < static_cast<uint64_t>(k_in) && below + c2[y] >= static_cast<uint64_t>(k_in)) {
-          sh.bin = 2 * tid + y;
-          sh.before = below;
-          sh.total = below + c2[y];
+          sh.said[0] = 2 * tid + y;
+          sh.said[1] = below;
+          sh.said[2] = below + c2[y];
         }
         below += c2[y];
       }
-      __syncthreads();
-      const int bin = sh.bin;
-      const uint64_t before = sh.before, through = bin < 0 ? all : sh.total;
-      if (through <= kList) {
-        gather(0.f, bin < 0 ? ends : bin + 1.f, 0);
-        finish_list(static_cast<int>(through), k_in);
-        return;
-      }
-      if (bin >= 0) {
-        const uint64_t left = k_in - before;
-        if (through - before <= kList) {
-          const int len = gather(static_cast<float>(bin), bin + 1.f, 0);
-          if (rank == 0) {
-            sort_list(sh.list, len);
-            if (tid == 0) sh.cut = sh.list[left - 1], sh.n_list = 0;
-          }
-          cluster.sync();
-          cut = *cluster.map_shared_rank(&sh.cut, 0);
-        } else {
-          cut = bisect([&](float) -> uint64_t { return 1; }, static_cast<float>(bin), bin + 1.f, 0, left);
-        }
+    }
+    uint64_t v[3];
+    learn(v);
+    const bool some = v[0] < kBins;  // else fewer than k weigh anything
+    const float lo = static_cast<float>(v[0]), hi = some ? lo + 1.f : ends;
+    if (v[2] <= kList) {
+      const int len = gather(0.f, hi, 0);
+      finish_list(len, hi, k_in);
+      return;
+    }
+    if (some) {
+      const uint64_t left = k_in - v[1];
+      if (v[2] - v[1] <= kList) {
+        const int len = gather(lo, hi, 0);
+        if (rank == 0) sh.said[0] = cut_list(len, lo, hi, 0, left, false);
+        learn(v);
+        cut = v[0];
+      } else {
+        cut = bisect([&](float) -> uint64_t { return 1; }, lo, hi, 0, left);
       }
     }
   }
   if (use_p) {
-    if (use_k) cluster.sync();  // sh.cut has been read
+    if (use_k && rank == 0) {  // the finer bins were there
+      __syncthreads();
+      sh.lo[tid] = sh.hi[tid] = sh.lo[tid + kThreads] = sh.hi[tid + kThreads] = 0;
+      __syncthreads();
+    }
     for (int q = tid; q < quads; q += kThreads) {
       float f[4];
       get4(q, f);
+      uint64_t w[4];
+      uint32_t old[4];
+      int at[4];
+      // the four's adds are on their way together
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const float x = r.place(f[y]);
-        if (!(x < ends && f[y] > -INFINITY) || (cut && rank_key(f[y], i0 + 4 * q + y) < cut)) continue;
-        const uint64_t w = weight(r.e(f[y]));
-        const int at = bin_of(x);
-        const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&sh.lo[at], l);
-        const uint32_t h = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
-        if (h) atomicAdd(&sh.hi[at], h);
+        const bool in = x < ends && f[y] > -INFINITY && (!cut || rank_key(f[y], i0 + 4 * q + y) >= cut);
+        w[y] = in ? weight(r.e(f[y])) : 0;
+        at[y] = bin_of(x);
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) old[y] = w[y] ? atomicAdd(&sh.lo[at[y]], static_cast<uint32_t>(w[y])) : 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t h = static_cast<uint32_t>(w[y] >> 32) + (old[y] + static_cast<uint32_t>(w[y]) < old[y] ? 1u : 0u);
+        if (h) atomicAdd(&sh.hi[at[y]], h);
       }
     }
     cluster.sync();
-    uint64_t w2[2] = {};
+    if (rank == 0) {
+      uint64_t w2[2] = {};
 #pragma unroll 8
-    for (int c = 0; c < kMaxCluster; ++c)
-      if (c < C) {
-        const uint2 l = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.lo, c) + 2 * tid);
-        const uint2 h = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.hi, c) + 2 * tid);
-        w2[0] += static_cast<uint64_t>(h.x) << 32 | l.x;
-        w2[1] += static_cast<uint64_t>(h.y) << 32 | l.y;
-      }
-    uint64_t total;
-    uint64_t below = block_before(w2[0] + w2[1], sh.warp64, total);
-    const uint64_t bar = top_p_bar(top_p, total);
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      if (below < bar && below + w2[y] >= bar) {  // exactly one bin
-        sh.bin = 2 * tid + y;
-        sh.before = below;
-      }
-      below += w2[y];
-    }
-    __syncthreads();
-    const int bin = sh.bin;
-    const uint64_t before = sh.before;
-    const int in_bin = gather(static_cast<float>(bin), bin + 1.f, cut);
-    if (in_bin <= kList) {
-      if (rank == 0) {
-        sort_list(sh.list, in_bin);
-        constexpr int kEach = kList / kThreads;
-        uint64_t w[kEach], sum = 0, unused;
-#pragma unroll
-        for (int y = 0; y < kEach; ++y) {
-          const int x = tid * kEach + y;
-          w[y] = x < in_bin ? weight(r.e(key_logit(sh.list[x]))) : 0;
-          sum += w[y];
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < C) {
+          const uint2 l = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.lo, c) + 2 * tid);
+          const uint2 h = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.hi, c) + 2 * tid);
+          w2[0] += static_cast<uint64_t>(h.x) << 32 | l.x;
+          w2[1] += static_cast<uint64_t>(h.y) << 32 | l.y;
         }
-        uint64_t at = before + block_before(sum, sh.warp64, unused);
+      uint64_t total;
+      uint64_t below = block_before(w2[0] + w2[1], sh.warp64, total);
+      const uint64_t bar = top_p_bar(top_p, total);
 #pragma unroll
-        for (int y = 0; y < kEach; ++y) {
-          if (at < bar && at + w[y] >= bar) sh.cut = sh.list[tid * kEach + y];
-          at += w[y];
+      for (int y = 0; y < 2; ++y) {
+        if (below < bar && below + w2[y] >= bar) {  // exactly one bin
+          sh.said[0] = 2 * tid + y;
+          sh.said[1] = bar - below;
         }
+        below += w2[y];
       }
-      cluster.sync();
-      cut = *cluster.map_shared_rank(&sh.cut, 0);
-    } else {
-      cut = bisect([&](float v) { return weight(r.e(v)); }, static_cast<float>(bin), bin + 1.f, cut, bar - before);
     }
+    uint64_t v[3];
+    learn(v);
+    const float lo = static_cast<float>(v[0]);
+    const uint64_t need = v[1];
+    const int len = gather(lo, lo + 1.f, cut);
+    if (rank == 0) {
+      const uint64_t key = len <= kList ? cut_list(len, lo, lo + 1.f, cut, need, true) : 0;
+      if (tid == 0) sh.said[0] = key;
+    }
+    learn(v);
+    cut = v[0] ? v[0] : bisect([&](float x) { return weight(r.e(x)); }, lo, lo + 1.f, cut, need);
   }
 
   // 5: each warp a contiguous part of the CTA's range
@@ -725,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   cluster.sync();  // the neighbours' shared memory stays until all have read it
 }
 
-// CTAs a row: eight where the rows alone fill the GPU, up to sixteen where they do not.
+// CTAs a row: doubled while the rows' CTAs are no more than the SMs, and so many that a CTA's range takes at most 96 KB
+// (64 rows of 92,544: 24.2 us with four CTAs a row, one an SM; 26.6 with eight, two an SM in two waves).
 template <int DT>
 int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
   static int most[64] = {};  // the largest cluster that the device places
@@ -753,7 +826,9 @@ int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
     most[dev] = fit > 0 ? kMaxCluster : 8;
   }
   int c = 1;
-  while (c < most[dev] && p.V > c * 2048 && (p.B * c < ctx->num_sms || p.V / c > 24000)) c *= 2;
+  while (c < most[dev] && p.V > c * 2048 &&
+         (static_cast<int64_t>(p.B) * c <= ctx->num_sms || p.V / c * static_cast<int64_t>(sizeof(typename Raw<DT>::Type)) > 96000))
+    c *= 2;
   p.per = (p.V + c - 1) / c;
   const int size = static_cast<int>(sizeof(typename Raw<DT>::Type)), fixed = static_cast<int>(align16(sizeof(Shared)));
   const int room = (ctx->max_smem_optin - fixed) / size / 16 * 16, want = (p.per + 31) / 16 * 16;  // its ends' padding too
