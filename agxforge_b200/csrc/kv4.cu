@@ -25,7 +25,7 @@ struct AppendParams {
   const __half* kn;
   float eps, qscale;
   void* q;
-  int q_bf16;
+  int q_bf16, vec;  // vec = every row, table and vector is aligned to four values
   unsigned* err;
 };
 
@@ -34,6 +34,27 @@ __device__ __forceinline__ float load1(const void* p, int64_t i) {
   if (DT == AGXC_F32) return static_cast<const float*>(p)[i];
   if (DT == AGXC_F16) return __half2float(static_cast<const __half*>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// four values from index i on, in one load where they are aligned to their size together
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, int64_t i, bool vec, float* x) {
+  if (!vec) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = load1<DT>(p, i + e);
+    return;
+  }
+  if constexpr (DT == AGXC_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t h = ((e & 2 ? v.y : v.x) >> (16 * (e & 1))) & 0xffffu;
+      x[e] = DT == AGXC_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16);
+    }
+  }
 }
 
 // min and max over the LPH lanes of a head
@@ -51,136 +72,156 @@ __device__ __forceinline__ unsigned code4(float x, float s, float b) {
   return isfinite(q) ? static_cast<unsigned>(fminf(fmaxf(q, 0.f), 15.f)) : 0u;
 }
 
-// hd / 4 lanes a head: lane l holds dims 2l, 2l + 1 and the dims hd / 2 above them (a RoPE pair each, and one code byte
-// each). A warp takes one head of 128 or two of 64.
+// hd / 8 lanes a head: lane l holds dims 4l .. 4l + 3 and the dims hd / 2 above them (four RoPE pairs, two code bytes
+// side by side each). A warp takes two heads of 128 or four of 64.
+// Every value is read once and each lane's loads, codes and q are one access each; 3,585 tokens of 14 + 2 x 2 heads of 64
+// with the read back of their rows: 11.6 us (single values a lane took 14.0), where the bytes alone, 18.6 MB, take 2.8: what
+// is left are two launches and one wave of short chains, load, exchange over the head's lanes, divide, store. One token: 3.9.
 template <int HD, int DT>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
   using Tile = Kv4Tile<HD>;
-  constexpr int LPH = HD / 4;
-  const int heads = p.H + 2 * p.c.kvh;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LPH;
+  constexpr int LPH = HD / 8;
+  pdl_enter(1);
+  const unsigned heads = p.H + 2 * p.c.kvh, item = blockIdx.x * (256 / LPH) + threadIdx.x / LPH;
   const int l = threadIdx.x % LPH;
-  const bool live = item < static_cast<int64_t>(p.T) * heads;
-  const int t = live ? static_cast<int>(item / heads) : 0, head = live ? static_cast<int>(item % heads) : 0;
+  const bool live = item < p.T * heads;
+  const int t = live ? item / heads : 0, head = live ? item - t * heads : 0;
+  const bool is_q = head < p.H, is_v = head >= p.H + p.c.kvh;
+  float x[8];
+  const int d0 = 4 * l, d1 = HD / 2 + 4 * l;
+  const int64_t row = static_cast<int64_t>(t) * p.ld + head * HD;
+  load4<DT>(p.qkv, row + d0, p.vec, x);
+  load4<DT>(p.qkv, row + d1, p.vec, x + 4);
   const int pos = p.pos[t];
   const int64_t slot = p.slots[t];
-  const bool is_q = head < p.H, is_v = head >= p.H + p.c.kvh;
   const bool bad = pos < 0 || pos >= p.table_rows || slot >= static_cast<int64_t>(p.c.pages) * p.c.page;
-  if (live && bad && l == 0 && p.err) atomicOr(p.err, kErrBadPos);
-  float x[4];
-  const int d0 = 2 * l, d1 = HD / 2 + 2 * l;
-  const int64_t row = static_cast<int64_t>(t) * p.ld + static_cast<int64_t>(head) * HD;
-  x[0] = load1<DT>(p.qkv, row + d0);
-  x[1] = load1<DT>(p.qkv, row + d0 + 1);
-  x[2] = load1<DT>(p.qkv, row + d1);
-  x[3] = load1<DT>(p.qkv, row + d1 + 1);
+  if (live && bad && l == 0) atomicOr(p.err, kErrBadPos);
+  float cs[4], sn[4];
+  if (!is_v && !bad) {
+    load4<AGXC_F32>(p.cos_t, static_cast<int64_t>(pos) * (HD / 2) + d0, p.vec, cs);
+    load4<AGXC_F32>(p.sin_t, static_cast<int64_t>(pos) * (HD / 2) + d0, p.vec, sn);
+  }
   if (p.bias) {
-    const __half* b = p.bias + static_cast<int64_t>(head) * HD;
-    x[0] = __fadd_rn(x[0], __half2float(b[d0]));
-    x[1] = __fadd_rn(x[1], __half2float(b[d0 + 1]));
-    x[2] = __fadd_rn(x[2], __half2float(b[d1]));
-    x[3] = __fadd_rn(x[3], __half2float(b[d1 + 1]));
+    float b[8];
+    load4<AGXC_F16>(p.bias, head * HD + d0, p.vec, b);
+    load4<AGXC_F16>(p.bias, head * HD + d1, p.vec, b + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(x[e], b[e]);
   }
   if (p.qn) {
-    float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
 #pragma unroll
     for (int m = LPH / 2; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
     if (!is_v) {
       const float r = rsqrtf(sum / static_cast<float>(HD) + p.eps);
       const __half* g = is_q ? p.qn : p.kn;
-      x[0] = (x[0] * r) * __half2float(g[d0]);
-      x[1] = (x[1] * r) * __half2float(g[d0 + 1]);
-      x[2] = (x[2] * r) * __half2float(g[d1]);
-      x[3] = (x[3] * r) * __half2float(g[d1 + 1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (x[e] * r) * __half2float(g[e < 4 ? d0 + e : d1 + e - 4]);
     }
   }
   if (!is_v && !bad) {
-    const float* c = p.cos_t + static_cast<int64_t>(pos) * (HD / 2);
-    const float* s = p.sin_t + static_cast<int64_t>(pos) * (HD / 2);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x1 = x[e], x2 = x[2 + e], cc = c[d0 + e], ss = s[d0 + e];
-      x[e] = __fadd_rn(__fmul_rn(x1, cc), -__fmul_rn(x2, ss));
-      x[2 + e] = __fadd_rn(__fmul_rn(x2, cc), __fmul_rn(x1, ss));
+    for (int e = 0; e < 4; ++e) {
+      const float x1 = x[e], x2 = x[4 + e];
+      x[e] = __fadd_rn(__fmul_rn(x1, cs[e]), -__fmul_rn(x2, sn[e]));
+      x[4 + e] = __fadd_rn(__fmul_rn(x2, cs[e]), __fmul_rn(x1, sn[e]));
     }
   }
   // the shuffles below are the whole warp's
-  float lo0 = fminf(x[0], x[1]), hi0 = fmaxf(x[0], x[1]), lo1 = fminf(x[2], x[3]), hi1 = fmaxf(x[2], x[3]);
-  if (HD == 64) {
-    lo0 = fminf(lo0, lo1);
-    hi0 = fmaxf(hi0, hi1);
+  float lo[2], hi[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    lo[h] = fminf(fminf(x[4 * h], x[4 * h + 1]), fminf(x[4 * h + 2], x[4 * h + 3]));
+    hi[h] = fmaxf(fmaxf(x[4 * h], x[4 * h + 1]), fmaxf(x[4 * h + 2], x[4 * h + 3]));
   }
-  head_minmax<LPH>(lo0, hi0);
-  if (HD == 128) head_minmax<LPH>(lo1, hi1);
+  if (HD == 64) {
+    lo[0] = lo[1] = fminf(lo[0], lo[1]);
+    hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
+  }
+  head_minmax<LPH>(lo[0], hi[0]);
+  if (HD == 128) head_minmax<LPH>(lo[1], hi[1]);
   if (!live || bad) return;
   if (is_q) {
-    const int64_t o = (static_cast<int64_t>(t) * p.H + head) * HD;
+    uint16_t* o = static_cast<uint16_t*>(p.q) + (static_cast<int64_t>(t) * p.H + head) * HD;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t at = o + (e < 2 ? d0 + e : d1 + e - 2);
-      const float v = __fmul_rn(x[e], p.qscale);
-      if (p.q_bf16) static_cast<__nv_bfloat16*>(p.q)[at] = __float2bfloat16_rn(v);
-      else static_cast<__half*>(p.q)[at] = __float2half_rn(v);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float a = __fmul_rn(x[4 * h + 2 * e], p.qscale), b = __fmul_rn(x[4 * h + 2 * e + 1], p.qscale);
+        if (p.q_bf16) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+          w[e] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __half2 v = __floats2half2_rn(a, b);
+          w[e] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      *reinterpret_cast<uint2*>(o + (h ? d1 : d0)) = make_uint2(w[0], w[1]);
     }
     return;
   }
   if (slot < 0) return;
   const int j = is_v ? head - p.H - p.c.kvh : head - p.H;
-  const int page = static_cast<int>(slot / p.c.page), off = static_cast<int>(slot % p.c.page), tt = off & 15;
+  const int page = static_cast<int>(quotient(slot, p.c.page));
+  const int off = static_cast<int>(slot - static_cast<int64_t>(page) * p.c.page), tt = off & 15;
   uint8_t* tile = Tile::ptr(p.c, page, j, off >> 4);
 #pragma unroll
-  for (int pr = 0; pr < 2; ++pr) {
-    const int g = HD == 128 ? pr : 0, i = HD == 128 ? l : pr * 16 + l;
-    const float lo = g ? lo1 : lo0, hi = g ? hi1 : hi0;
-    const __half sh = __float2half_rn(hi > lo ? __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f) : 1.f), bh = __float2half_rn(lo);
+  for (int h = 0; h < 2; ++h) {
+    const int g = HD == 128 ? h : 0, i = HD == 128 ? 2 * l : h * 16 + 2 * l;
+    const float low = HD == 128 ? lo[h] : lo[0], high = HD == 128 ? hi[h] : hi[0];
+    const __half sh = __float2half_rn(high > low ? __fmul_rn(__fsub_rn(high, low), 1.f / 15.f) : 1.f);
+    const __half bh = __float2half_rn(low);
     const float s = __half2float(sh), b = __half2float(bh);
-    const unsigned byte = code4(x[2 * pr], s, b) | code4(x[2 * pr + 1], s, b) << 4;
-    tile[is_v ? Tile::v_at(tt, g, i) : Tile::k_at(tt, g, i)] = static_cast<uint8_t>(byte);
-    if (l == 0 && (HD == 128 || pr == 0))
+    unsigned two = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) two |= code4(x[4 * h + e], s, b) << (4 * e);
+    *reinterpret_cast<uint16_t*>(tile + (is_v ? Tile::v_at(tt, g, i) : Tile::k_at(tt, g, i))) = static_cast<uint16_t>(two);
+    if (l == 0 && (HD == 128 || h == 0))
       *reinterpret_cast<__half2*>(tile + Tile::kSb + tt * Tile::kEntry + (is_v ? 4 * Tile::G : 0) + 4 * g) =
           __halves2half2(sh, bh);
   }
 }
 
-// One thread per (token, KV head, K or V, byte pair of dims): two adjacent dims of one code byte.
+// One thread per (token, KV head, K or V, two bytes of codes): four adjacent dims.
 template <int HD>
 __global__ void __launch_bounds__(256) rows_kernel(Kv4 c, const int64_t* __restrict__ slots, int T,
                                                    __half* __restrict__ k, __half* __restrict__ v, unsigned* err) {
   using Tile = Kv4Tile<HD>;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t all = static_cast<int64_t>(T) * c.kvh * HD;  // (HD / 2) bytes x (K, V)
-  if (i >= all) return;
-  const int byte = static_cast<int>(i % (HD / 2)), is_v = static_cast<int>(i / (HD / 2) % 2);
-  const int64_t th = i / HD;
-  const int t = static_cast<int>(th / c.kvh), j = static_cast<int>(th % c.kvh);
+  pdl_enter(1);
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, th = i / (HD / 2);  // hd / 4 threads each of K and V
+  const int four = i % (HD / 4), is_v = i / (HD / 4) % 2, t = th / c.kvh, j = th - t * c.kvh;
+  if (t >= T) return;
   const int64_t slot = slots[t];
-  __half2 out = __float2half2_rn(0.f);
+  __half2 out[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
   if (slot >= static_cast<int64_t>(c.pages) * c.page) {
-    if (err) atomicOr(err, kErrBadPos);
+    atomicOr(err, kErrBadPos);
   } else if (slot >= 0) {
-    const int page = static_cast<int>(slot / c.page), off = static_cast<int>(slot % c.page), tt = off & 15;
+    const int page = static_cast<int>(quotient(slot, c.page));
+    const int off = static_cast<int>(slot - static_cast<int64_t>(page) * c.page), tt = off & 15;
     const uint8_t* tile = Tile::ptr(c, page, j, off >> 4);
-    const int g = byte >> 5, b = byte & 31;
-    const unsigned code = tile[is_v ? Tile::v_at(tt, g, b) : Tile::k_at(tt, g, b)];
+    const int g = four >> 4, b = 2 * (four & 15);
+    const unsigned code = *reinterpret_cast<const uint16_t*>(tile + (is_v ? Tile::v_at(tt, g, b) : Tile::k_at(tt, g, b)));
     const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(tile + Tile::kSb + tt * Tile::kEntry +
                                                                        (is_v ? 4 * Tile::G : 0) + 4 * g));
-    out = __floats2half2_rn(__fmaf_rn(static_cast<float>(code & 15), sb.x, sb.y),
-                            __fmaf_rn(static_cast<float>(code >> 4), sb.x, sb.y));
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      out[e] = __floats2half2_rn(__fmaf_rn(static_cast<float>(code >> (8 * e) & 15), sb.x, sb.y),
+                                 __fmaf_rn(static_cast<float>(code >> (8 * e + 4) & 15), sb.x, sb.y));
   }
-  reinterpret_cast<__half2*>(is_v ? v : k)[th * (HD / 2) + byte] = out;
+  uint2 w = make_uint2(*reinterpret_cast<uint32_t*>(&out[0]), *reinterpret_cast<uint32_t*>(&out[1]));
+  *reinterpret_cast<uint2*>((is_v ? v : k) + static_cast<int64_t>(th) * HD + 4 * four) = w;
 }
 
 template <int HD>
 int append_launch(const AppendParams& p, cudaStream_t s) {
-  const int64_t items = static_cast<int64_t>(p.T) * (p.H + 2 * p.c.kvh);
-  const int64_t grid = (items * (HD / 4) + 255) / 256;
-  if (grid > 0x7fffffff) return fail(AGXC_EINVAL, "kv4_append: too many tokens for one call");
-  const dim3 g(static_cast<unsigned>(grid));
-  if (p.dtype == AGXC_F32) append_kernel<HD, AGXC_F32><<<g, 256, 0, s>>>(p);
-  else if (p.dtype == AGXC_F16) append_kernel<HD, AGXC_F16><<<g, 256, 0, s>>>(p);
-  else append_kernel<HD, AGXC_BF16><<<g, 256, 0, s>>>(p);
-  AGXC_CUDA(cudaGetLastError());
-  return 0;
+  const int per = 256 / (HD / 8);
+  const dim3 g(static_cast<unsigned>((static_cast<int64_t>(p.T) * (p.H + 2 * p.c.kvh) + per - 1) / per));
+  if (p.dtype == AGXC_F32) return launch_ex(append_kernel<HD, AGXC_F32>, g, dim3(256), 0, s, 1, p);
+  if (p.dtype == AGXC_F16) return launch_ex(append_kernel<HD, AGXC_F16>, g, dim3(256), 0, s, 1, p);
+  return launch_ex(append_kernel<HD, AGXC_BF16>, g, dim3(256), 0, s, 1, p);
 }
 
 }  // namespace
@@ -216,6 +257,9 @@ AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* a, v
   if (a->tokens == 0) return 0;
   if (!a->qkv_dev || !a->positions_dev || !a->slots_dev || !a->cos_dev || !a->sin_dev || !a->q_dev)
     return fail(AGXC_EINVAL, "kv4_append: null buffer");
+  if (reinterpret_cast<uintptr_t>(a->q_dev) % 8) return fail(AGXC_EINVAL, "kv4_append: q must be 8-byte aligned");
+  if (static_cast<int64_t>(a->tokens) * (a->heads + 2 * a->cache.kv_heads) > 0x7fffffff)
+    return fail(AGXC_EINVAL, "kv4_append: too many tokens for one call");
   AppendParams p;
   p.c = kv4_of(a->cache);
   p.qkv = a->qkv_dev; p.ld = a->qkv_ld; p.dtype = a->qkv_dtype; p.T = a->tokens; p.H = a->heads;
@@ -225,6 +269,10 @@ AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* a, v
   p.qn = reinterpret_cast<const __half*>(a->q_norm_dev);
   p.kn = reinterpret_cast<const __half*>(a->k_norm_dev);
   p.eps = a->eps; p.qscale = a->qscale; p.q = a->q_dev; p.q_bf16 = a->q_dtype == AGXC_BF16; p.err = ctx->err_dev;
+  const int size = a->qkv_dtype == AGXC_F32 ? 16 : 8;  // bytes of four values
+  p.vec = reinterpret_cast<uintptr_t>(a->qkv_dev) % size == 0 && a->qkv_ld % 4 == 0 &&
+          reinterpret_cast<uintptr_t>(a->cos_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(a->sin_dev) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(a->bias_dev) % 8 == 0;
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   return a->cache.head_dim == 128 ? append_launch<128>(p, s) : append_launch<64>(p, s);
 }
@@ -237,15 +285,16 @@ AGXC_API int agxc_kv4_rows_dev(agxc_ctx* ctx, const agxc_kv4_cache* cache, const
   if (tokens == 0) return 0;
   if (!slots_dev || !k_dev || !v_dev) return fail(AGXC_EINVAL, "kv4_rows: null buffer");
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  const int64_t n = static_cast<int64_t>(tokens) * cache->kv_heads * cache->head_dim, grid = (n + 255) / 256;
-  if (grid > 0x7fffffff) return fail(AGXC_EINVAL, "kv4_rows: too many tokens for one call");
-  const dim3 g(static_cast<unsigned>(grid));
+  if (reinterpret_cast<uintptr_t>(k_dev) % 8 || reinterpret_cast<uintptr_t>(v_dev) % 8)
+    return fail(AGXC_EINVAL, "kv4_rows: k and v must be 8-byte aligned");
+  const int64_t n = static_cast<int64_t>(tokens) * cache->kv_heads * cache->head_dim / 2;
+  if (n > 0x7fffffff - 256) return fail(AGXC_EINVAL, "kv4_rows: too many tokens for one call");
+  const dim3 g(static_cast<unsigned>((n + 255) / 256));
   __half* k = reinterpret_cast<__half*>(k_dev);
   __half* v = reinterpret_cast<__half*>(v_dev);
-  if (cache->head_dim == 128) rows_kernel<128><<<g, 256, 0, s>>>(kv4_of(*cache), slots_dev, tokens, k, v, ctx->err_dev);
-  else rows_kernel<64><<<g, 256, 0, s>>>(kv4_of(*cache), slots_dev, tokens, k, v, ctx->err_dev);
-  AGXC_CUDA(cudaGetLastError());
-  return 0;
+  return cache->head_dim == 128
+             ? launch_ex(rows_kernel<128>, g, dim3(256), 0, s, 1, kv4_of(*cache), slots_dev, tokens, k, v, ctx->err_dev)
+             : launch_ex(rows_kernel<64>, g, dim3(256), 0, s, 1, kv4_of(*cache), slots_dev, tokens, k, v, ctx->err_dev);
 }
 
 }  // extern "C"

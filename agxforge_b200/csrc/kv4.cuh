@@ -7,6 +7,11 @@
 
 namespace agxc {
 
+// a / b for 0 <= a, 0 < b, in 32 bits where that does
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
 struct Kv4 {
   uint8_t* data = nullptr;
   int pages = 0, kvh = 0, page = 0;  // page = tokens a page

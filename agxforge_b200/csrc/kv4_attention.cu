@@ -85,11 +85,6 @@ struct Place {
   }
 };
 
-// a / b for 0 <= a, 0 < b, in 32 bits where that does
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return ((a | b) >> 32) ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
-}
-
 // Blocks a CTA: the line's length over the CTAs. Every warp computes it for itself.
 __device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane) {
   long long sum = 0;
