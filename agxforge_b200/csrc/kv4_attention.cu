@@ -25,7 +25,9 @@
 // instead, whose CTAs join their pieces in shared memory: one launch, and no second kernel to wait for.
 #include <cooperative_groups.h>
 
-#include "kv4.cuh"
+#include <atomic>
+
+#include "kv4_attention.cuh"
 
 namespace agxc {
 namespace {
@@ -36,29 +38,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;   // of the warps that compute; one more warp copies
 constexpr int kBlock = 32 * kWarps;     // keys a block
 constexpr float kNone = -1e30f;         // the maximum that stands for no key
-
-struct Kv4AttnParams {
-  Kv4 c;
-  const void* q;
-  void* out;
-  int B, n, H, G, CB;                   // G = q heads a KV head, CB = column blocks an item row
-  int table_ld, max_pages;
-  int ctas, cluster;                    // cluster = CTAs an item, 0 = the line
-  const int32_t* table;
-  const int32_t* lengths;
-  float* part;                          // [2 ctas][columns]{max, sum}, then [2 ctas][columns][hd]
-  unsigned* err;
-};
-
-__device__ __forceinline__ int seq_len(const Kv4AttnParams& p, int b) {
-  const int len = p.lengths[b];
-  const int most = p.max_pages * p.c.page;
-  if (len < 0 || len > most) {
-    atomicOr(p.err, kErrBadPos);
-    return len < 0 ? 0 : most;
-  }
-  return len;
-}
 
 __device__ __forceinline__ int blocks_of(int len) { return (len + kBlock - 1) / kBlock; }
 
@@ -78,7 +57,7 @@ struct Place {
           rem = 0;
           return;
         }
-        len = seq_len(p, b);
+        len = kv4_seq_len(p, b);
         T = blocks_of(len);
       } while (T == 0);
     }
@@ -88,7 +67,7 @@ struct Place {
 // Blocks a CTA: the line's length over the CTAs. Every warp computes it for itself.
 __device__ __forceinline__ long long line_quota(const Kv4AttnParams& p, int lane) {
   long long sum = 0;
-  for (int b = lane; b < p.B; b += 32) sum += blocks_of(seq_len(p, b));
+  for (int b = lane; b < p.B; b += 32) sum += blocks_of(kv4_seq_len(p, b));
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   sum *= p.c.kvh * p.CB;
@@ -102,7 +81,7 @@ __device__ __forceinline__ bool line_find(const Kv4AttnParams& p, int lane, long
   const int items = p.c.kvh * p.CB;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const int l = b < p.B ? seq_len(p, b) : 0;
+    const int l = b < p.B ? kv4_seq_len(p, b) : 0;
     const long long mine = static_cast<long long>(blocks_of(l)) * items;
     long long up = mine;
 #pragma unroll
@@ -123,32 +102,14 @@ __device__ __forceinline__ bool line_find(const Kv4AttnParams& p, int lane, long
   return false;
 }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // a barrier of the warps that compute
 __device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
-__device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
 
 // code - 8 of the even (hi = 0) or 16 (code - 8) of the odd nibble in the low byte of each half of x, times 2^-24 (an
 // exact difference of fp16 subnormals)
@@ -168,41 +129,6 @@ __device__ __forceinline__ void mma_zero(float* d, uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.f));
-}
-
-__device__ __forceinline__ void unpack8(const uint4& u, float* f, const __half*) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = bits_float2(w[i]);
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
-}
-__device__ __forceinline__ void unpack8(const uint4& u, float* f, const __nv_bfloat16*) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* f);
-template <>
-__device__ __forceinline__ uint4 pack8<__half>(const float* f) {
-  return make_uint4(half2_bits(f[0], f[1]), half2_bits(f[2], f[3]), half2_bits(f[4], f[5]), half2_bits(f[6], f[7]));
-}
-template <>
-__device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Shared memory of a CTA: stages of a block's tiles, the warps' results [warp][column][hd + 4], {max, sum} of each, the
@@ -239,13 +165,6 @@ __device__ __forceinline__ void join16(float m, float sum, float* v) {
   }
 }
 
-template <int HD, typename T>
-__device__ __forceinline__ void write8(const Kv4AttnParams& p, int b, int j, int col, int d, const float* v) {
-  T* dst = static_cast<T*>(p.out) +
-           ((static_cast<long long>(b) * p.n + col / p.G) * p.H + j * p.G + col % p.G) * HD + d;
-  *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
-}
-
 template <int HD, int NT, typename T, bool CL>
 __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
@@ -276,7 +195,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     const int unit = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
     at.b = unit / (p.c.kvh * p.CB);
     at.item = unit % (p.c.kvh * p.CB);
-    at.len = seq_len(p, at.b);
+    at.len = kv4_seq_len(p, at.b);
     at.T = blocks_of(at.len);
     const int per = (at.T + p.cluster - 1) / p.cluster;
     at.t = rank * per;
@@ -682,7 +601,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        write8<HD, T>(p, at.b, j, col0 + col, d, v);
+        kv4_write8<HD, T>(p, at.b, j, col0 + col, d, v);
       } else if (CL) {                       // this thread's own place among the first warp's results
         float* dst = so + col * Sm::kRow + d;
         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
@@ -717,7 +636,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         v[4] = e.x; v[5] = e.y; v[6] = e.z; v[7] = e.w;
       }
       join16(ml.x, ml.y, v);
-      if (x == 0 && u0 + (lane >> 4) < units) write8<HD, T>(p, cl_b, j, col0 + col, d, v);
+      if (x == 0 && u0 + (lane >> 4) < units) kv4_write8<HD, T>(p, cl_b, j, col0 + col, d, v);
     }
     cluster.sync();                          // the neighbours' shared memory stays until all have read it
   }
@@ -734,13 +653,13 @@ __global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid
   // The lengths may be read before the first kernel is done: it let this one start after its own wait. What follows in
   // the stream may start to start: it waits for this kernel's end.
   pdl_launch_dependents();
-  const int blocks = blocks_of(seq_len(p, b));
+  const int blocks = blocks_of(kv4_seq_len(p, b));
   const int j = item / p.CB, col0 = item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
   long long c0 = 0, c1 = 0;
   if (blocks) {
     const long long quota = line_quota(p, lane);
     long long before = 0;
-    for (int x = lane; x < b; x += 32) before += blocks_of(seq_len(p, x));
+    for (int x = lane; x < b; x += 32) before += blocks_of(kv4_seq_len(p, x));
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) before += __shfl_xor_sync(0xffffffffu, before, m);
     const long long start = before * items + static_cast<long long>(item) * blocks;
@@ -777,7 +696,7 @@ __global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid
       const float inv = t.sum > 0.f ? 1.f / t.sum : 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) t.v[e] *= inv;
-      write8<HD, T>(p, b, j, col0 + col, d, t.v);
+      kv4_write8<HD, T>(p, b, j, col0 + col, d, t.v);
     }
     return;
   }
@@ -787,7 +706,7 @@ __global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid
     Sum t;
     for (long long x = c0 + (lane & 15); x <= c1; x += 16) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
     join16(t.m, t.sum, t.v);
-    if ((lane & 15) == 0 && u0 + (lane >> 4) < units) write8<HD, T>(p, b, j, col0 + col, d, t.v);
+    if ((lane & 15) == 0 && u0 + (lane >> 4) < units) kv4_write8<HD, T>(p, b, j, col0 + col, d, t.v);
   }
 }
 
@@ -807,67 +726,130 @@ int attn_check(const agxc_kv4_attention_args* a) {
   return 0;
 }
 
-// The launch's shape: 16 columns a block where one row's heads do not fill 8. Up to an eighth as many items as the GPU
-// holds CTAs (three an SM with 8 columns, two with 16): a cluster each, of as many CTAs as fit, at most 16 or one a block
-// of the longest sequence possible. More: the line, over all CTAs that the GPU holds at once. (1 x 1,792 tokens of 8 KV
-// heads: 12.4 us as a line of 112 CTAs and its join, 7.0 as clusters; the line balances what the clusters cannot, unequal
-// lengths, where they have few CTAs each.)
+// A kernel's attributes, set once a device; the device, or a negative error.
+template <int HD, int NT, typename T, bool CL>
+int attn_device() {
+  static std::atomic<bool> allowed[64] = {};
+  int dev = 0;
+  AGXC_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64) return fail(AGXC_EINVAL, "kv4_attention: device index below 64");
+  if (!allowed[dev]) {
+    auto* kernel = kv4_attn_kernel<HD, NT, T, CL>;
+    AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NT>::kBytes));
+    if (CL) AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    allowed[dev] = true;
+  }
+  return dev;
+}
+
+template <int HD, int NT>
+cudaLaunchConfig_t attn_config(int ctas, int cluster, cudaStream_t s, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads + 32);
+  cfg.dynamicSmemBytes = Smem<HD, NT>::kBytes;
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+// How many clusters of 2^log2 CTAs run at once, as the runtime says it; negative on an error.
+template <int HD, int NT, typename T>
+int attn_fit(int log2) {
+  static std::atomic<int> fit[64][5] = {};  // one more than the clusters, 0 = not asked yet
+  const int dev = attn_device<HD, NT, T, true>();
+  if (dev < 0) return dev;
+  int n = fit[dev][log2];
+  if (!n) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = attn_config<HD, NT>(1 << log2, 1 << log2, nullptr, attr);
+    cfg.numAttrs = 1;
+    AGXC_CUDA(cudaOccupancyMaxActiveClusters(&n, kv4_attn_kernel<HD, NT, T, true>, &cfg));
+    fit[dev][log2] = ++n;
+  }
+  return n - 1;
+}
+
+// The launch's shape: 16 columns a block where one row's heads do not fill 8. Where clusters of four CTAs (or of as many
+// as the longest sequence possible has blocks) run for all items at once: a cluster an item, of as many CTAs as do, 16 at
+// most. More items than that: the line, over all CTAs that the GPU holds at once, or, from 64 columns a KV head on, the
+// kernel of many rows.
+//   1 x 1,792 tokens, 8 items of 8 columns: 6.7 us as clusters, 12.4 as a line. 64 items of 8 columns, 8 x 1,807: 12.6 as
+//   clusters, 13.7 as a line; ragged 11.7 and 14.7; 8 x 8,192: 31.0 and 27.8. The line balances unequal lengths, but is two
+//   launches, and its join has few CTAs where there are few items (8 x 64 blocks: 10.2 as clusters, 21.7 as a line). One
+//   cluster more than run at once costs a second wave: 16 items of 16 columns took 22.4 us in clusters of 16, 14.5 of 8.
+//   8 x 1,807 ragged of 8 KV heads, columns a head: 32 as a line 26.6, in the other kernel 31.2; 64: 41.6 and 32.0; 128: 62.8
+//   and 33.8. 1 x 1,807, 64 columns (32 items): 15.6 as clusters here, 20.9 there.
 struct Shape {
   int nt, cb, ctas, cluster;
-  int64_t bytes(int hd) const { return cluster ? 0 : static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
+  bool chunk;
+  int64_t bytes(int hd) const { return cluster || chunk ? 0 : static_cast<int64_t>(ctas) * 2 * (8 * nt) * (hd + 2) * 4; }
 };
 
-Shape attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
-  Shape s;
+template <int HD, int NT, typename T>
+int attn_cluster(const agxc_ctx* ctx, int64_t items, int64_t longest, int& size) {
+  size = 0;
+  for (int x = 0; x <= 4 && 1 << x <= ctx->max_cluster && (x == 0 || (1 << x) < 2 * longest); ++x) {
+    if (longest > 1 && items << x > 4 * ctx->num_sms) break;  // no more than four CTAs an SM: not asked for
+    const int most = longest <= 1 ? 0x7fffffff : attn_fit<HD, NT, T>(x);
+    if (most < 0) return most;
+    if (items > most) break;
+    size = 1 << x;
+  }
+  if (size < 4 && size < longest) size = 0;
+  return 0;
+}
+
+int attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a, Shape& s) {
   const int64_t cols = static_cast<int64_t>(a->rows) * (a->heads / a->cache.kv_heads);
   s.nt = cols > 8 ? 2 : 1;
   s.cb = static_cast<int>((cols + 8 * s.nt - 1) / (8 * s.nt));
   const int64_t items = static_cast<int64_t>(a->batch) * a->cache.kv_heads * s.cb;
   const int64_t most = static_cast<int64_t>(a->max_pages) * a->cache.page_size;
   const int64_t longest = (most + kBlock - 1) / kBlock, full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
-  s.cluster = 0;
-  if (items * 8 <= full || (longest <= 1 && items <= 0x7fffffff)) {
-    s.cluster = 1;
-    while (s.cluster < ctx->max_cluster && s.cluster < 16 && s.cluster < longest && items * s.cluster * 2 <= full) s.cluster *= 2;
+  s.chunk = false;
+  s.ctas = 0;
+  const bool bf16 = a->dtype == AGXC_BF16;
+  int rc;
+  if (a->cache.head_dim == 128)
+    rc = s.nt == 1 ? bf16 ? attn_cluster<128, 1, __nv_bfloat16>(ctx, items, longest, s.cluster)
+                          : attn_cluster<128, 1, __half>(ctx, items, longest, s.cluster)
+                   : bf16 ? attn_cluster<128, 2, __nv_bfloat16>(ctx, items, longest, s.cluster)
+                          : attn_cluster<128, 2, __half>(ctx, items, longest, s.cluster);
+  else
+    rc = s.nt == 1 ? bf16 ? attn_cluster<64, 1, __nv_bfloat16>(ctx, items, longest, s.cluster)
+                          : attn_cluster<64, 1, __half>(ctx, items, longest, s.cluster)
+                   : bf16 ? attn_cluster<64, 2, __nv_bfloat16>(ctx, items, longest, s.cluster)
+                          : attn_cluster<64, 2, __half>(ctx, items, longest, s.cluster);
+  if (rc) return rc;
+  if (s.cluster) {
     s.ctas = static_cast<int>(items * s.cluster);
-    return s;
+    return 0;
   }
+  s.chunk = cols >= 64;
+  if (s.chunk) return 0;
   const int64_t blocks = items * longest;
   s.ctas = static_cast<int>(blocks < full ? blocks : full);
-  return s;
+  return 0;
 }
 
 template <int HD, int NT, typename T, bool CL>
 int attn_launch(const Kv4AttnParams& p, cudaStream_t s) {
-  constexpr int smem = Smem<HD, NT>::kBytes;
-  static bool allowed[64] = {};
-  int dev = 0;
-  AGXC_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64) return fail(AGXC_EINVAL, "kv4_attention: device index below 64");
+  if (const int dev = attn_device<HD, NT, T, CL>(); dev < 0) return dev;
   auto* kernel = kv4_attn_kernel<HD, NT, T, CL>;
-  if (!allowed[dev]) {
-    AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (CL) AGXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    allowed[dev] = true;
-  }
   if (CL) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.ctas);
-    cfg.blockDim = dim3(kThreads + 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    const cudaLaunchConfig_t cfg = attn_config<HD, NT>(p.ctas, p.cluster, s, attr);
     AGXC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return 0;
   }
-  if (int rc = launch_ex(kernel, dim3(p.ctas), dim3(kThreads + 32), smem, s, 1, p)) return rc;
+  if (int rc = launch_ex(kernel, dim3(p.ctas), dim3(kThreads + 32), Smem<HD, NT>::kBytes, s, 1, p)) return rc;
   return launch_ex(kv4_join_kernel<HD, NT, T>, dim3(static_cast<unsigned>(p.B) * p.c.kvh * p.CB), dim3(64 * NT), 0, s, 1,
                    p);
 }
@@ -888,7 +870,10 @@ extern "C" {
 AGXC_API int64_t agxc_kv4_attention_workspace(agxc_ctx* ctx, const agxc_kv4_attention_args* a) {
   if (!ctx) return fail(AGXC_EINVAL, "kv4_attention: null context");
   if (attn_check(a)) return -1;
-  return attn_shape(ctx, a).bytes(a->cache.head_dim);
+  if (a->batch == 0 || a->rows == 0) return 0;
+  Shape sh;
+  if (attn_shape(ctx, a, sh)) return -1;
+  return sh.bytes(a->cache.head_dim);
 }
 
 AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args* a, void* stream) {
@@ -899,7 +884,8 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
     return fail(AGXC_EINVAL, "kv4_attention: null buffer");
   if (reinterpret_cast<uintptr_t>(a->q_dev) % 16 || reinterpret_cast<uintptr_t>(a->out_dev) % 16)
     return fail(AGXC_EINVAL, "kv4_attention: q and out must be 16-byte aligned");
-  const Shape sh = attn_shape(ctx, a);
+  Shape sh;
+  if (int rc = attn_shape(ctx, a, sh)) return rc;
   const int64_t need = sh.bytes(a->cache.head_dim);
   if (need && (a->workspace_bytes < need || !a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16))
     return fail(AGXC_EINVAL, "kv4_attention: a 16-byte aligned workspace of agxc_kv4_attention_workspace bytes");
@@ -911,6 +897,7 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
   p.part = static_cast<float*>(a->workspace_dev); p.err = ctx->err_dev;
   cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const bool bf16 = a->dtype == AGXC_BF16;
+  if (sh.chunk) return launch_kv4_chunk(ctx, p, a->cache.head_dim, bf16, s);
   if (a->cache.head_dim == 128)
     return bf16 ? attn_launch_shape<128, __nv_bfloat16>(p, sh, s) : attn_launch_shape<128, __half>(p, sh, s);
   return bf16 ? attn_launch_shape<64, __nv_bfloat16>(p, sh, s) : attn_launch_shape<64, __half>(p, sh, s);

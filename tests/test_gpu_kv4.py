@@ -296,6 +296,80 @@ def test_attention(torch, lens, n, H, KVH, hd, page, dtype, kind):
         _check(torch, last, q[:, -1:], seqs, lens)
 
 
+@pytest.mark.parametrize("lens,n,H,KVH,hd,page,dtype,kind", [
+    ([0, 1, 130, 64, 257], 96, 16, 8, 128, 64, "fp16", "normal"),   # rows before the sequence begins, one key
+    ([2049], 80, 16, 8, 128, 16, "fp16", "normal"),                  # an item's keys over a cluster, a second block of columns
+    ([333], 100, 14, 2, 64, 48, "bf16", "normal"),                   # pages that end inside a block of keys
+    ([512], 512, 16, 8, 64, 16, "fp16", "normal"),                   # a prompt from its first token
+    ([70, 3, 71, 200, 64, 128, 1, 90] * 3, 70, 8, 8, 128, 32, "fp16", "normal"),
+    ([300, 90], 65, 40, 1, 64, 16, "bf16", "normal"),                # forty heads on one KV head
+    ([900, 40], 77, 32, 8, 128, 64, "fp16", "peaks"),
+    ([900, 140], 150, 14, 2, 64, 64, "bf16", "peaks"),
+    ([600, 40], 64, 32, 8, 128, 64, "fp16", "spread"),
+    ([600, 40], 64, 32, 8, 64, 64, "fp16", "spread"),
+    ([600], 64, 32, 8, 128, 64, "bf16", "tiny"),
+    ([200], 64, 32, 8, 128, 64, "fp16", "flat"),
+    ([200], 64, 32, 8, 128, 64, "bf16", "small q"),
+])
+def test_attention_many_rows(torch, lens, n, H, KVH, hd, page, dtype, kind):
+    from agxforge.kernels import kv4
+    rng = np.random.default_rng(len(lens) * 100 + n + hd)
+    dt = torch.float16 if dtype == "fp16" else torch.bfloat16
+    cache, table, q, seqs = _case(torch, rng, lens, n, H, KVH, hd, page, dt, kind)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = kv4.attention(q, cache, table, lt)
+    kv4.check_errors()
+    _check(torch, out, q, seqs, lens)
+    assert torch.equal(out, kv4.attention(q, cache, table, lt))
+    # the rows of a chunk one by one, as single tokens see them
+    last = kv4.attention(q[:, -1], cache, table, lt)
+    _check(torch, last[:, None], q[:, -1:], seqs, lens)
+
+
+def test_attention_many_rows_bad_lengths_and_pages(torch):
+    from agxforge.kernels import kv4
+    rng = np.random.default_rng(19)
+    lens = [128, 128]
+    cache, table, q, seqs = _case(torch, rng, lens, 100, 32, 8, 128, 64, torch.float16)
+    table = table[:, :2].contiguous()
+    out = kv4.attention(q, cache, table, torch.tensor([128, 1 << 30], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="out of range"):
+        kv4.check_errors()
+    _check(torch, out, q, seqs, lens)
+    out = kv4.attention(q, cache, table, torch.tensor([128, -5], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="out of range"):
+        kv4.check_errors()
+    assert bool((out[1] == 0).all())
+    _check(torch, out[:1], q[:1], seqs[:1], lens[:1])
+    for page in (-1, cache.pages):                                    # pages outside the cache: no keys from them
+        t2 = table.clone()
+        t2[1] = page
+        out = kv4.attention(q, cache, t2, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+        with pytest.raises(RuntimeError, match="out of range"):
+            kv4.check_errors()
+        _check(torch, out[:1], q[:1], seqs[:1], lens[:1])
+        assert bool((out[1] == 0).all())
+
+
+def test_attention_many_rows_in_a_graph(torch):
+    """Captured once, replayed with other lengths."""
+    from agxforge.kernels import kv4
+    rng = np.random.default_rng(14)
+    lens = [400, 190]
+    cache, table, q, seqs = _case(torch, rng, lens, 64, 32, 8, 128, 64, torch.float16)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kv4.attention(q, cache, table, lt)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = kv4.attention(q, cache, table, lt)
+    for cut in ([400, 190], [17, 64]):
+        lt.copy_(torch.tensor(cut, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        _check(torch, out, q, [(K[:L], V[:L], [p[:L] for p in pr]) for (K, V, pr), L in zip(seqs, cut)], cut)
+
+
 def test_attention_far_pages(torch):
     """Pages past 4 GiB of a cache: byte offsets beyond 32 bits."""
     from agxforge.kernels import kv4
