@@ -16,6 +16,14 @@
 //   4  where a bin holds a cut, only that bin is listed. The key the cut falls on: 1,024 finer bins, then a comparison of
 //      the few elements of one of them. A bin that is more than a list (thousands of equal logits) is cut bit by bit
 //   5  the kept weights' total and the token, in index order: the warp, then the element, that the target falls on
+//
+// 256 rows of 151,936 fp32 logits (155.6 MB, 23.8 us at the copy rate), eight CTAs a row, 37 rows at a time: 55 us greedy,
+// 122 with the weights alone, 146 with top-k 50, 310 with top-p 0.95, 194 where rows mix all of these. The SMs bind it, not
+// DRAM: a wave of top-p rows takes 5 us to load and find the maximum, 9.6 for the weights in bins (an exp and a shared-memory
+// add each), 3.6 for the first CTA to add the cluster's bins up, 4.4 to list the cut's bin, 2.7 to cut, 4.9 for the kept
+// weights and 2 for the draw, and the cluster's barriers between them leave warps waiting. One row with top-k 50: 13.8 us,
+// steps and barriers; 64 rows of 92,544 with min-p: 24.2; 33 rows of 50,257 bf16, top-k 1,000: 28.4. Sorting the listed keys
+// in place of finer bins took 382 for the top-p rows and 43 for the 33.
 #include <cooperative_groups.h>
 
 #include <cfloat>

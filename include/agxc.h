@@ -207,7 +207,7 @@ typedef struct {
   const uint16_t* q_norm_dev; /* fp16 [head_dim]: RMS norm of each q (k) head before RoPE; both or neither */
   const uint16_t* k_norm_dev;
   float eps, qscale;          /* the norm's epsilon; the factor on q after RoPE (log2(e) / sqrt(head_dim)) */
-  void* q_dev;                /* [tokens][heads][head_dim], fp16 or bf16 */
+  void* q_dev;                /* [tokens][heads][head_dim], fp16 or bf16, 8-byte aligned */
   int32_t q_dtype;            /* AGXC_F16 or AGXC_BF16 */
 } agxc_kv4_append_args;
 
@@ -216,14 +216,15 @@ typedef struct {
  * (kErrBadPos) and leaves that token out. tokens = 0 does nothing. */
 AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* args, void* stream);
 
-/* The values the cache holds at `tokens` slots, fp16 [tokens][kv_heads][head_dim] each (zeros for a negative slot). */
+/* The values the cache holds at `tokens` slots, fp16 [tokens][kv_heads][head_dim] each, 8-byte aligned (zeros for a
+ * negative slot). */
 AGXC_API int agxc_kv4_rows_dev(agxc_ctx* ctx, const agxc_kv4_cache* cache, const int64_t* slots_dev, int tokens,
                                uint16_t* k_dev, uint16_t* v_dev, void* stream);
 
 typedef struct {
   agxc_kv4_cache cache;
   const void* q_dev;          /* [batch][rows][heads][head_dim], scaled for the base-2 softmax; fp16 or bf16 */
-  void* out_dev;              /* the same shape and type */
+  void* out_dev;              /* the same shape and type; both 16-byte aligned */
   int32_t dtype;              /* AGXC_F16 or AGXC_BF16 */
   int32_t batch, rows, heads;
   const int32_t* page_table_dev; /* [batch][table_ld]: page of each page_size tokens of a sequence */
@@ -243,7 +244,7 @@ typedef struct {
   const void* logits_dev;     /* [batch][logits_ld] */
   int64_t logits_ld;
   int32_t dtype;              /* AGXC_F32, _F16, _BF16 */
-  int32_t batch, vocab;
+  int32_t batch, vocab;       /* vocab at most 1,048,576, batch at most 67,108,864 */
   const float* u_dev;         /* [batch] uniform numbers in [0, 1) */
   float temperature, top_p, min_p; /* used where the array below is NULL */
   int32_t top_k;
