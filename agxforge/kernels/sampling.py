@@ -31,7 +31,7 @@ def _option(v, dtype, B, index, name):
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Tokens int32 [batch] and their probabilities fp32 [batch] for logits [batch, vocab] fp32, fp16 or bf16 (rows may
-    be strided) and u fp32 [batch] in [0, 1). temperature, top_p and min_p: numbers or fp32 [batch]; top_k: a number or
+    be strided, vocab at most 1,048,576) and u fp32 [batch] in [0, 1). temperature, top_p and min_p: numbers or fp32 [batch]; top_k: a number or
     int32 [batch]."""
     kind, idx = DTYPES.get(logits.dtype), logits.get_device()
     if logits.dim() != 2 or kind is None or idx < 0 or logits.shape[1] < 1 or \

@@ -223,3 +223,14 @@ def test_refuses(torch):
             sampling.sample(*args)
     token, prob = sampling.sample(x[:0], u[:0])
     assert token.shape == (0,) and prob.shape == (0,)
+
+
+def test_refuses_a_vocabulary_past_the_limit(torch):
+    from agxforge.kernels.sampling import sample
+    u = torch.zeros(1, device="cuda")
+    with pytest.raises(ValueError, match="1,048,576"):
+        sample(torch.zeros(1, (1 << 20) + 1, device="cuda"), u)
+    x = torch.zeros(1, 1 << 20, dtype=torch.float16, device="cuda")
+    x[0, (1 << 20) - 1] = 40.0                                        # all the weight on the last index
+    token, prob = sample(x, u + 0.5)
+    assert int(token) == (1 << 20) - 1 and abs(float(prob) - 1.0) <= 2.0 ** -18
