@@ -13,17 +13,19 @@
 //      each CTA its own, and the first CTA collects them and finishes the row
 //   3  top-p: the bins' exact weights (64 bits as two 32-bit shared-memory adds, the second with the first's carry, rarely
 //      needed); the bin that holds the bar
-//   4  where a bin holds a cut, only that bin is listed. The key the cut falls on: 1,024 finer bins, then a comparison of
-//      the few elements of one of them. A bin that is more than a list (thousands of equal logits) is cut bit by bit
+//   4  where a bin holds a cut, only that bin is listed (and for top-p the weights above it are added up in the same pass).
+//      The key the cut falls on: 1,024 finer bins, then a comparison of the few elements of one of them. A bin that is more
+//      than a list (thousands of equal logits) is cut bit by bit
 //   5  the kept weights' total and the token, in index order: the warp, then the element, that the target falls on
 //
 // 256 rows of 151,936 fp32 logits (155.6 MB, 23.8 us at the copy rate), eight CTAs a row, 37 rows at a time: 55 us greedy,
-// 122 with the weights alone, 146 with top-k 50, 310 with top-p 0.95, 194 where rows mix all of these. The SMs bind it, not
-// DRAM: a wave of top-p rows takes 5 us to load and find the maximum, 9.6 for the weights in bins (an exp and a shared-memory
-// add each), 3.6 for the first CTA to add the cluster's bins up, 4.4 to list the cut's bin, 2.7 to cut, 4.9 for the kept
-// weights and 2 for the draw, and the cluster's barriers between them leave warps waiting. One row with top-k 50: 13.8 us,
-// steps and barriers; 64 rows of 92,544 with min-p: 24.2; 33 rows of 50,257 bf16, top-k 1,000: 28.4. Sorting the listed keys
-// in place of finer bins took 382 for the top-p rows and 43 for the 33.
+// 122 with the weights alone, 145 with top-k 50, 283 with top-p 0.95, 187 where rows mix all of these. The SMs bind it, not
+// DRAM (fetching the next rows into L2 meanwhile gained nothing): of a top-p row's time 5 us go to loading it and its
+// maximum, 9.6 to the weights in bins (an exp and a shared-memory add each), 3.6 to the first CTA's sum of the cluster's
+// bins, 6 to the list of the cut's bin and the weights above it, 2.7 to the cut and 2 to the draw, and the cluster's
+// barriers between them leave warps waiting. One row with top-k 50: 13.8 us, steps and barriers; 64 rows of 92,544 with
+// min-p: 24.2; 33 rows of 50,257 bf16, top-k 1,000: 28. Not kept: the listed keys sorted in place of finer bins (382 for
+// the top-p rows, 43 for the 33), a pass of their own for the kept weights (310).
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -383,25 +385,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
     for (int x = 0; x < 3; ++x) v[x] = __shfl_sync(0xffffffffu, o, x);
   };
-  // Lists the elements at places from `lo` to below `hi` whose keys reach `from`; returns their number over the cluster,
-  // all of them in the first CTA's list where they fit, to that CTA.
-  auto gather = [&](float lo, float hi, uint64_t from) {
-    __syncthreads();
-    if (tid == 0) sh.n_list = 0;
-    __syncthreads();
-    for (int q = tid; q < quads; q += kThreads) {
-      float f[4];
-      get4(q, f);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float at = r.place(f[y]);
-        if (!(at >= lo && at < hi && f[y] > -INFINITY)) continue;
-        const uint64_t key = rank_key(f[y], i0 + 4 * q + y);
-        if (key < from) continue;
-        const int x = atomicAdd(&sh.n_list, 1);
-        if (x < kList) sh.list[x] = key;
-      }
-    }
+  // The lists' length over the cluster, all of them in the first CTA's list where they fit, to that CTA.
+  auto collect = [&]() {
     cluster.sync();
     int len = 0;
     if (rank == 0) {  // a warp for each CTA's list, behind this one's own
@@ -421,6 +406,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       __syncthreads();
     }
     return len;
+  };
+  // Lists the elements at places from `lo` to below `hi` whose keys reach `from`, and collects them.
+  auto gather = [&](float lo, float hi, uint64_t from) {
+    __syncthreads();
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    for (int q = tid; q < quads; q += kThreads) {
+      float f[4];
+      get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float at = r.place(f[y]);
+        if (!(at >= lo && at < hi && f[y] > -INFINITY)) continue;
+        const uint64_t key = rank_key(f[y], i0 + 4 * q + y);
+        if (key < from) continue;
+        const int x = atomicAdd(&sh.n_list, 1);
+        if (x < kList) sh.list[x] = key;
+      }
+    }
+    return collect();
   };
   // In the first CTA: the key among the list's first `len`, all at places from `lo` to below `hi`, from which up those
   // that reach `from` sum to `need`, by number or by weight.
@@ -619,6 +624,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
 
   uint64_t cut = 0;  // keys from `cut` up are kept
+  // each warp has a contiguous part of the CTA's range where weights are added up
+  const int part = (quads + kWarps - 1) / kWarps, q0 = min(quads, warp * part), q1 = min(quads, q0 + part);
+  bool summed = false;  // the parts' kept weights are there
   if (use_k) {
     for (int q = tid; q < quads; q += kThreads) {
       float f[4];
@@ -682,22 +690,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int q = tid; q < quads; q += kThreads) {
       float f[4];
       get4(q, f);
-      uint64_t w[4];
-      uint32_t old[4];
+      uint32_t hi[4], lo[4], old[4];
       int at[4];
       // the four's adds are on their way together
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const float x = r.place(f[y]);
         const bool in = x < ends && f[y] > -INFINITY && (!cut || rank_key(f[y], i0 + 4 * q + y) >= cut);
-        w[y] = in ? weight(r.e(f[y])) : 0;
+        // the weight's two words: 2^15 + e rounded towards zero has floor(2^8 e) in its low bits, and what that leaves is exact
+        const float e = in ? r.e(f[y]) : 0.f, t = __fadd_rz(e, 32768.f);
+        hi[y] = __float_as_uint(t) - 0x47000000u;
+        lo[y] = __float2uint_rz(__fmul_rn(__fsub_rn(e, __fsub_rn(t, 32768.f)), 1099511627776.f));
         at[y] = bin_of(x);
       }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) old[y] = w[y] ? atomicAdd(&sh.lo[at[y]], static_cast<uint32_t>(w[y])) : 0;
+      for (int y = 0; y < 4; ++y) old[y] = lo[y] ? atomicAdd(&sh.lo[at[y]], lo[y]) : 0;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const uint32_t h = static_cast<uint32_t>(w[y] >> 32) + (old[y] + static_cast<uint32_t>(w[y]) < old[y] ? 1u : 0u);
+        const uint32_t h = hi[y] + (old[y] + lo[y] < old[y] ? 1u : 0u);
         if (h) atomicAdd(&sh.hi[at[y]], h);
       }
     }
@@ -728,33 +738,70 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     learn(v);
     const float lo = static_cast<float>(v[0]);
     const uint64_t need = v[1];
-    const int len = gather(lo, lo + 1.f, cut);
+    // In one pass: the bin's elements are listed, and the weights of those above it, which are kept, added up.
+    __syncthreads();
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    WeightSum above;
+    for (int q = q0 + lane; q < q1; q += 32) {
+      float f[4];
+      get4(q, f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float at = r.place(f[y]), e = r.e(f[y]);
+        above.add(at < lo && e >= min_p ? e : 0.f);
+        if (!(at >= lo && at < lo + 1.f && f[y] > -INFINITY)) continue;
+        const uint64_t key = rank_key(f[y], i0 + 4 * q + y);
+        if (key < cut) continue;
+        const int x = atomicAdd(&sh.n_list, 1);
+        if (x < kList) sh.list[x] = key;
+      }
+    }
+    const uint64_t sum = warp_sum64(above.get());
+    if (lane == 0) sh.warp_kept[warp] = sum;
+    int len = collect();
     if (rank == 0) {
       const uint64_t key = len <= kList ? cut_list(len, lo, lo + 1.f, cut, need, true) : 0;
       if (tid == 0) sh.said[0] = key;
     }
     learn(v);
-    cut = v[0] ? v[0] : bisect([&](float x) { return weight(r.e(x)); }, lo, lo + 1.f, cut, need);
+    summed = v[0] != 0;
+    if (summed) {  // and the kept of the bin, each to its part
+      cut = v[0];
+      if (rank > 0) len = sh.n_list;
+      for (int x = tid; x < len; x += kThreads) {
+        const uint64_t key = sh.list[x];
+        const int i = key_index(key);
+        const float e = r.e(key_logit(key));
+        if (key >= cut && i >= r0 && i < r0 + n && e >= min_p)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.warp_kept[((i - i0) >> 2) / part]),
+                    static_cast<unsigned long long>(weight(e)));
+      }
+    } else {
+      cut = bisect([&](float x) { return weight(r.e(x)); }, lo, lo + 1.f, cut, need);
+    }
   }
 
-  // 5: each warp a contiguous part of the CTA's range
+  // 5: the parts' kept weights, and the part, the thread's fours and the element that the target falls on
   const float cut_v = cut ? key_logit(cut) : -INFINITY;  // kept: above the cut's logit, or equal and not after its index
   const int cut_i = cut ? key_index(cut) : 0x7fffffff;
   auto kept_e = [&](float v, int i) {
     const float e = r.e(v);
     return e >= min_p && (v > cut_v || (v == cut_v && i <= cut_i)) ? e : 0.f;
   };
-  const int part = (quads + kWarps - 1) / kWarps, q0 = min(quads, warp * part), q1 = min(quads, q0 + part);
-  WeightSum ws;
+  if (!summed) {
+    WeightSum ws;
 #pragma unroll 2
-  for (int q = q0 + lane; q < q1; q += 32) {
-    float f[4];
-    get4(q, f);
+    for (int q = q0 + lane; q < q1; q += 32) {
+      float f[4];
+      get4(q, f);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) ws.add(kept_e(f[y], i0 + 4 * q + y));
+      for (int y = 0; y < 4; ++y) ws.add(kept_e(f[y], i0 + 4 * q + y));
+    }
+    const uint64_t own = warp_sum64(ws.get());
+    if (lane == 0) sh.warp_kept[warp] = own;
   }
-  uint64_t sum = warp_sum64(ws.get());
-  if (lane == 0) sh.warp_kept[warp] = sum;
+  uint64_t sum;
   __syncthreads();
   if (tid == 0) {
     sum = 0;
