@@ -116,9 +116,10 @@ def append(cache, qkv, positions, slots, cos, sin, heads, bias=None, q_norm=None
     width = (heads + 2 * cache.kv_heads) * hd
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError("append: heads a positive multiple of kv_heads")
-    if qkv.dim() != 2 or qkv.shape[1] != width:
+    shape = qkv.shape
+    if len(shape) != 2 or shape[1] != width:
         raise ValueError("append: qkv is [tokens, (heads + 2 kv_heads) * head_dim] = [tokens, %d]" % width)
-    T = qkv.shape[0]
+    T = shape[0]
     ld, inner = qkv.stride()
     kind = DTYPES.get(qkv.dtype)
     if kind is None or qkv.get_device() != idx or inner != 1:
@@ -129,7 +130,8 @@ def append(cache, qkv, positions, slots, cos, sin, heads, bias=None, q_norm=None
         raise ValueError("append: one position and one slot a token")
     _check(cos, torch.float32, idx, "append: cos")
     _check(sin, torch.float32, idx, "append: sin")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or cos.shape[0] < 1:
+    shape = cos.shape
+    if len(shape) != 2 or shape != sin.shape or shape[1] != hd // 2 or shape[0] < 1:
         raise ValueError("append: cos and sin are [n, head_dim / 2]")
     if bias is not None:
         _check(bias, torch.float16, idx, "append: bias")
@@ -144,16 +146,18 @@ def append(cache, qkv, positions, slots, cos, sin, heads, bias=None, q_norm=None
             q_dtype = torch.bfloat16 if kind == N.BF16 else torch.float16
         _need(q_dtype is torch.float16 or q_dtype is torch.bfloat16, "append: q fp16 or bf16")
         out = torch.empty(T, heads, hd, dtype=q_dtype, device=cache.device)
+        q_kind = DTYPES[q_dtype]
     else:
         _need(out.dtype in (torch.float16, torch.bfloat16), "append: q fp16 or bf16")
         _check(out, out.dtype, idx, "append: out")
         _need(out.shape == (T, heads, hd), "append: out is [tokens, heads, head_dim]")
+        q_kind = DTYPES[out.dtype]
     if qscale is None:
         qscale = _QSCALE[hd]
     a = N.Kv4AppendArgs(cache._c, qkv.data_ptr(), ld if T > 1 else width, kind, T, heads, positions.data_ptr(),
-                        slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                        slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), shape[0],
                         None if bias is None else bias.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
-                        None if k_norm is None else k_norm.data_ptr(), eps, qscale, out.data_ptr(), DTYPES[out.dtype])
+                        None if k_norm is None else k_norm.data_ptr(), eps, qscale, out.data_ptr(), q_kind)
     rc = N.lib().agxc_kv4_append_dev(N.context(idx), C.byref(a), _stream(idx))
     if rc:
         N.check(rc, "append")
@@ -178,8 +182,9 @@ def attention(q, cache, page_table, lengths, out=None):
     _check(lengths, torch.int32, idx, "attention: lengths")
     if lengths.numel() != B:
         raise ValueError("attention: one length a sequence")
-    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype is not torch.int32 or \
-            page_table.get_device() != idx or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+    pages = page_table.shape
+    if len(pages) != 2 or pages[0] != B or page_table.dtype is not torch.int32 or \
+            page_table.get_device() != idx or (page_table.stride(1) != 1 and pages[1] > 1):
         raise ValueError("attention: page_table int32 [batch, max_pages] on the cache's device, its rows contiguous")
     if not q.is_contiguous():
         q = q.contiguous()
@@ -188,7 +193,7 @@ def attention(q, cache, page_table, lengths, out=None):
     else:
         _check(out, q.dtype, idx, "attention: out")
         _need(out.shape == shape, "attention: out has q's shape")
-    mp = page_table.shape[1]
+    mp = pages[1]
     a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), kind, B, n, H, page_table.data_ptr(),
                            page_table.stride(0) if B > 1 else mp, mp, lengths.data_ptr(), None, 0)
     L, ctx = N.lib(), N.context(idx)

@@ -22,7 +22,7 @@ from agxforge.kernels.kv4 import DTYPES, _stream
 
 def _option(v, dtype, B, index, name):
     """(number, device pointer): a number for all rows, or a tensor with one a row."""
-    if isinstance(v, torch.Tensor):
+    if type(v) is not float and type(v) is not int and isinstance(v, torch.Tensor):  # torch's own check takes a while
         if v.dtype is not dtype or v.get_device() != index or v.numel() != B or not v.is_contiguous():
             raise ValueError("sample: %s is a number or contiguous %s [batch] on the logits' device" % (name, str(dtype)[6:]))
         return 0, v.data_ptr()

@@ -195,8 +195,7 @@ def check(rc, what=""):
 
 def context(device=0):
     """The process's context on ``device`` (one stream per device)."""
-    with _lock:
-        h = _ctx.get(device)
+    h = _ctx.get(device)
     if h is None:
         L = lib()
         p = C.c_void_p()

@@ -245,6 +245,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (tid == 0) {
     for (int c = 0; c < kCopies; ++c) mbar_init(&sh.copied[c], 1);
     fence_mbar_init();
+    sh.n_list = 0;
+    sh.first = 0x7fffffff;
+  }
+  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.lo[x] = sh.hi[x] = 0;
+  pdl_wait();  // what came before is done from here on
+  pdl_launch_dependents();
+  if (tid == 0) {
     const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;
     for (int c = 0; c < kCopies; ++c) {
       const int at = min(bulk, c * each), len = min(bulk, at + each) - at;
@@ -259,8 +266,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (tail < nc) cache[pad + tail] = src[tail];
     else if (nc == n && pad + tail < 4 * quads) cache[pad + tail] = static_cast<T16>(kNaN<DT>);
   }
-  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.lo[x] = sh.hi[x] = 0;
-  if (tid == 0) sh.n_list = 0, sh.first = 0x7fffffff;
   const float T = fminf(p.T_a ? p.T_a[b] : p.T, FLT_MAX), top_p = p.p_a ? p.p_a[b] : p.top_p,
               min_p = p.m_a ? p.m_a[b] : p.min_p;
   const int k_in = p.k_a ? p.k_a[b] : p.top_k;
@@ -893,12 +898,14 @@ int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = fixed + size * static_cast<size_t>(p.cached);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = c;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   AGXC_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<DT>, p));
   return 0;
 }
