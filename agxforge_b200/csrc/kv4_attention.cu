@@ -29,8 +29,8 @@
 // 92.5). The SM's issue slots bind it, 59 of 100 taken at 12 warps an SM, with DRAM at 56: two ANDs, a subtraction and their
 // share of an MMA for each pair of codes of K and V, about 300 instructions a 16-key tile and warp where 475 took 197 us.
 // 128 ragged sequences of up to 1,792 tokens of 2 KV heads of 64 (18.6 MB): 18 us; one of 1,792 of 8: 6.7, both a launch, a
-// chain of three dependent loads and a join. 16 rows of 8 sequences: 26 to 31 us, the 32 columns a KV head as two blocks,
-// which dequantise each key twice. Not kept: compute warps that take the copy's turn (156 us), seven of them in two CTAs an
+// chain of three dependent loads and a join. 16 rows of 8 sequences: 23 us, the 32 columns a KV head as two blocks, which
+// dequantise each key twice. Not kept: compute warps that take the copy's turn (156 us), seven of them in two CTAs an
 // SM (136), codes or-ed into 1,024 (148).
 #include <cooperative_groups.h>
 
@@ -156,22 +156,27 @@ struct Smem {
   static constexpr int kBytes = kCame + kStages * 4;
 };
 
-// Sixteen lanes' results of one column's eight dims, {m, sum} and v each, as one: out on every lane.
-__device__ __forceinline__ void join16(float m, float sum, float* v) {
+// The results of `lanes` lanes (a power of two up to 16, lanes side by side) of one column's eight dims, {m, sum} and v
+// each, as one: out on each of them.
+__device__ __forceinline__ void join_lanes(int lanes, float m, float sum, float* v) {
   float mx = m;
 #pragma unroll
-  for (int x = 8; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  for (int x = 8; x >= 1; x >>= 1)
+    if (x < lanes) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
   const float f = ex2(m - mx);
   sum *= f;
 #pragma unroll
-  for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  for (int x = 8; x >= 1; x >>= 1)
+    if (x < lanes) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   const float inv = sum > 0.f ? f / sum : 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    v[e] *= inv;
+  for (int e = 0; e < 8; ++e) v[e] *= inv;
 #pragma unroll
-    for (int x = 8; x >= 1; x >>= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
-  }
+  for (int x = 8; x >= 1; x >>= 1)
+    if (x < lanes) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
+    }
 }
 
 template <int HD, int NT, typename T, bool CL>
@@ -633,19 +638,21 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     cluster.sync();
     const int rank = blockIdx.x % p.cluster, j = cl_item / p.CB, col0 = cl_item % p.CB * NC;
     const int units = min(NC, p.n * p.G - col0) * (HD / 8);
-    for (int u0 = (rank * kWarps + warp) * 2; warp < kWarps && u0 < units; u0 += p.cluster * kWarps * 2) {
-      const int u = min(u0 + (lane >> 4), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8, x = lane & 15;
-      float2 ml = make_float2(kNone, 0.f);
+    // a lane for each CTA's piece, so that a warp takes 32 / cluster units of eight dims at once (with sixteen lanes a unit
+    // whatever the cluster's size, one block of 16 columns in a cluster of one took 27 us; it takes 8)
+    const int lg = 31 - __clz(p.cluster), step = 32 >> lg;
+    for (int u0 = (rank * kWarps + warp) * step; warp < kWarps && u0 < units; u0 += p.cluster * kWarps * step) {
+      const int u = min(u0 + (lane >> lg), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8, x = lane & (p.cluster - 1);
       float v[8] = {};
-      if (x < p.cluster) ml = *cluster.map_shared_rank(reinterpret_cast<float2*>(sm + Sm::kOwn) + col, x);
+      const float2 ml = *cluster.map_shared_rank(reinterpret_cast<float2*>(sm + Sm::kOwn) + col, x);
       if (ml.y > 0.f) {
         const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(so + col * Sm::kRow + d, x));
         const float4 a = src[0], e = src[1];
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = e.x; v[5] = e.y; v[6] = e.z; v[7] = e.w;
       }
-      join16(ml.x, ml.y, v);
-      if (x == 0 && u0 + (lane >> 4) < units) kv4_write8<HD, T>(p, cl_b, j, col0 + col, d, v);
+      join_lanes(p.cluster, ml.x, ml.y, v);
+      if (x == 0 && u0 + (lane >> lg) < units) kv4_write8<HD, T>(p, cl_b, j, col0 + col, d, v);
     }
     cluster.sync();                          // the neighbours' shared memory stays until all have read it
   }
@@ -714,7 +721,7 @@ __global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid
     const int u = min(u0 + (lane >> 4), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8;
     Sum t;
     for (long long x = c0 + (lane & 15); x <= c1; x += 16) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
-    join16(t.m, t.sum, t.v);
+    join_lanes(16, t.m, t.sum, t.v);
     if ((lane & 15) == 0 && u0 + (lane >> 4) < units) kv4_write8<HD, T>(p, b, j, col0 + col, d, t.v);
   }
 }
@@ -787,14 +794,16 @@ int attn_fit(int log2) {
 
 // The launch's shape: 16 columns a block where one row's heads do not fill 8. Where clusters of four CTAs (or of as many
 // as the longest sequence possible has blocks) run for all items at once: a cluster an item, of as many CTAs as do, 16 at
-// most. More items than that: the line, over all CTAs that the GPU holds at once, or, from 64 columns a KV head on, the
-// kernel of many rows.
-//   1 x 1,792 tokens, 8 items of 8 columns: 6.7 us as clusters, 12.4 as a line. 64 items of 8 columns, 8 x 1,807: 12.6 as
-//   clusters, 13.7 as a line; ragged 11.7 and 14.7; 8 x 8,192: 31.0 and 27.8. The line balances unequal lengths, but is two
-//   launches, and its join has few CTAs where there are few items (8 x 64 blocks: 10.2 as clusters, 21.7 as a line). One
+// most. Clusters of two where these are three quarters of the CTAs that the GPU holds. More items than that: the line, over
+// all CTAs that the GPU holds at once, or, from 64 columns a KV head on, the kernel of many rows.
+//   1 x 1,792 tokens, 8 items of 8 columns: 6.7 us as clusters, 12.4 as a line. 64 items of 8 columns, 8 x 1,807: 12.8 as
+//   clusters, 13.7 as a line; ragged 11.8 and 14.7; 8 x 8,192: 31.3 and 27.8. The line balances unequal lengths, but is two
+//   launches, and its join has few CTAs where there are few items (8 x 64 blocks: 10.2 as clusters, 21.7 as a line).
+//   Clusters of two, items of 16 columns, 256 of 296 CTAs: 8 x 1,807 x 16 rows ragged 22.9, as a line 26.7; 8 x 8,192 66.0
+//   and 70.8; items of 8 columns, 256 of 444 CTAs: 16 x 8,192 55.0 and 43.9; 384 of 444: 24 x 1,807 16.4 and 21.5. One
 //   cluster more than run at once costs a second wave: 16 items of 16 columns took 22.4 us in clusters of 16, 14.5 of 8.
-//   8 x 1,807 ragged of 8 KV heads, columns a head: 32 as a line 26.6, in the other kernel 31.2; 64: 41.6 and 32.0; 128: 62.8
-//   and 33.8. 1 x 1,807, 64 columns (32 items): 15.6 as clusters here, 20.9 there.
+//   8 x 1,807 ragged of 8 KV heads, columns a head: 32 as clusters of two 22.9, in the other kernel 31.2; 64 as a line 41.6,
+//   there 32.0; 128: 62.8 and 33.8. 1 x 1,807 as clusters here and there: 64 columns (32 items) 14.0 and 20.9, 128 17.0 and 23.
 struct Shape {
   int nt, cb, ctas, cluster;
   bool chunk;
@@ -802,7 +811,7 @@ struct Shape {
 };
 
 template <int HD, int NT, typename T>
-int attn_cluster(const agxc_ctx* ctx, int64_t items, int64_t longest, int& size) {
+int attn_cluster(const agxc_ctx* ctx, int64_t cols, int64_t items, int64_t longest, int64_t full, int& size) {
   size = 0;
   for (int x = 0; x <= 4 && 1 << x <= ctx->max_cluster && (x == 0 || (1 << x) < 2 * longest); ++x) {
     if (longest > 1 && items << x > 4 * ctx->num_sms) break;  // no more than four CTAs an SM: not asked for
@@ -811,7 +820,8 @@ int attn_cluster(const agxc_ctx* ctx, int64_t items, int64_t longest, int& size)
     if (items > most) break;
     size = 1 << x;
   }
-  if (size < 4 && size < longest) size = 0;
+  const bool fills = size == 2 && cols < 64 && items * 8 >= full * 3;
+  if (size < 4 && size < longest && !fills) size = 0;
   return 0;
 }
 
@@ -827,15 +837,15 @@ int attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a, Shape& s) 
   const bool bf16 = a->dtype == AGXC_BF16;
   int rc;
   if (a->cache.head_dim == 128)
-    rc = s.nt == 1 ? bf16 ? attn_cluster<128, 1, __nv_bfloat16>(ctx, items, longest, s.cluster)
-                          : attn_cluster<128, 1, __half>(ctx, items, longest, s.cluster)
-                   : bf16 ? attn_cluster<128, 2, __nv_bfloat16>(ctx, items, longest, s.cluster)
-                          : attn_cluster<128, 2, __half>(ctx, items, longest, s.cluster);
+    rc = s.nt == 1 ? bf16 ? attn_cluster<128, 1, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
+                          : attn_cluster<128, 1, __half>(ctx, cols, items, longest, full, s.cluster)
+                   : bf16 ? attn_cluster<128, 2, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
+                          : attn_cluster<128, 2, __half>(ctx, cols, items, longest, full, s.cluster);
   else
-    rc = s.nt == 1 ? bf16 ? attn_cluster<64, 1, __nv_bfloat16>(ctx, items, longest, s.cluster)
-                          : attn_cluster<64, 1, __half>(ctx, items, longest, s.cluster)
-                   : bf16 ? attn_cluster<64, 2, __nv_bfloat16>(ctx, items, longest, s.cluster)
-                          : attn_cluster<64, 2, __half>(ctx, items, longest, s.cluster);
+    rc = s.nt == 1 ? bf16 ? attn_cluster<64, 1, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
+                          : attn_cluster<64, 1, __half>(ctx, cols, items, longest, full, s.cluster)
+                   : bf16 ? attn_cluster<64, 2, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
+                          : attn_cluster<64, 2, __half>(ctx, cols, items, longest, full, s.cluster);
   if (rc) return rc;
   if (s.cluster) {
     s.ctas = static_cast<int>(items * s.cluster);
