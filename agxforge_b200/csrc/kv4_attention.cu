@@ -795,7 +795,8 @@ int attn_fit(int log2) {
 // The launch's shape: 16 columns a block where one row's heads do not fill 8. Where clusters of four CTAs (or of as many
 // as the longest sequence possible has blocks) run for all items at once: a cluster an item, of as many CTAs as do, 16 at
 // most. Clusters of two where these are three quarters of the CTAs that the GPU holds. More items than that: the line, over
-// all CTAs that the GPU holds at once, or, from 64 columns a KV head on, the kernel of many rows.
+// all CTAs that the GPU holds at once, or, from 64 columns a KV head on (33 where no sequence is longer than a block), the
+// kernel of many rows.
 //   1 x 1,792 tokens, 8 items of 8 columns: 6.7 us as clusters, 12.4 as a line. 64 items of 8 columns, 8 x 1,807: 12.8 as
 //   clusters, 13.7 as a line; ragged 11.8 and 14.7; 8 x 8,192: 31.3 and 27.8. The line balances unequal lengths, but is two
 //   launches, and its join has few CTAs where there are few items (8 x 64 blocks: 10.2 as clusters, 21.7 as a line).
@@ -804,6 +805,8 @@ int attn_fit(int log2) {
 //   cluster more than run at once costs a second wave: 16 items of 16 columns took 22.4 us in clusters of 16, 14.5 of 8.
 //   8 x 1,807 ragged of 8 KV heads, columns a head: 32 as clusters of two 22.9, in the other kernel 31.2; 64 as a line 41.6,
 //   there 32.0; 128: 62.8 and 33.8. 1 x 1,807 as clusters here and there: 64 columns (32 items) 14.0 and 20.9, 128 17.0 and 23.
+//   60 sequences of at most 40 tokens, 128 columns a head: 118 as clusters of one, 45 there; 91 of 16, 48 columns: 66 and
+//   59; 235 of 6, 20 columns: 109 and 148.
 struct Shape {
   int nt, cb, ctas, cluster;
   bool chunk;
@@ -811,16 +814,17 @@ struct Shape {
 };
 
 template <int HD, int NT, typename T>
-int attn_cluster(const agxc_ctx* ctx, int64_t cols, int64_t items, int64_t longest, int64_t full, int& size) {
+int attn_cluster(const agxc_ctx* ctx, bool many, int64_t items, int64_t longest, int64_t full, int& size) {
   size = 0;
   for (int x = 0; x <= 4 && 1 << x <= ctx->max_cluster && (x == 0 || (1 << x) < 2 * longest); ++x) {
-    if (longest > 1 && items << x > 4 * ctx->num_sms) break;  // no more than four CTAs an SM: not asked for
-    const int most = longest <= 1 ? 0x7fffffff : attn_fit<HD, NT, T>(x);
+    const bool any = longest <= 1 && !many;  // an item is one block: CTAs in turn, without the line's second launch
+    if (!any && items << x > 4 * ctx->num_sms) break;  // no more than four CTAs an SM: not asked for
+    const int most = any ? 0x7fffffff : attn_fit<HD, NT, T>(x);
     if (most < 0) return most;
     if (items > most) break;
     size = 1 << x;
   }
-  const bool fills = size == 2 && cols < 64 && items * 8 >= full * 3;
+  const bool fills = size == 2 && !many && items * 8 >= full * 3;
   if (size < 4 && size < longest && !fills) size = 0;
   return 0;
 }
@@ -834,24 +838,24 @@ int attn_shape(const agxc_ctx* ctx, const agxc_kv4_attention_args* a, Shape& s) 
   const int64_t longest = (most + kBlock - 1) / kBlock, full = static_cast<int64_t>(ctx->num_sms) * (s.nt == 1 ? 3 : 2);
   s.chunk = false;
   s.ctas = 0;
-  const bool bf16 = a->dtype == AGXC_BF16;
+  const bool bf16 = a->dtype == AGXC_BF16, many = cols >= (longest <= 1 ? 33 : 64);
   int rc;
   if (a->cache.head_dim == 128)
-    rc = s.nt == 1 ? bf16 ? attn_cluster<128, 1, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
-                          : attn_cluster<128, 1, __half>(ctx, cols, items, longest, full, s.cluster)
-                   : bf16 ? attn_cluster<128, 2, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
-                          : attn_cluster<128, 2, __half>(ctx, cols, items, longest, full, s.cluster);
+    rc = s.nt == 1 ? bf16 ? attn_cluster<128, 1, __nv_bfloat16>(ctx, many, items, longest, full, s.cluster)
+                          : attn_cluster<128, 1, __half>(ctx, many, items, longest, full, s.cluster)
+                   : bf16 ? attn_cluster<128, 2, __nv_bfloat16>(ctx, many, items, longest, full, s.cluster)
+                          : attn_cluster<128, 2, __half>(ctx, many, items, longest, full, s.cluster);
   else
-    rc = s.nt == 1 ? bf16 ? attn_cluster<64, 1, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
-                          : attn_cluster<64, 1, __half>(ctx, cols, items, longest, full, s.cluster)
-                   : bf16 ? attn_cluster<64, 2, __nv_bfloat16>(ctx, cols, items, longest, full, s.cluster)
-                          : attn_cluster<64, 2, __half>(ctx, cols, items, longest, full, s.cluster);
+    rc = s.nt == 1 ? bf16 ? attn_cluster<64, 1, __nv_bfloat16>(ctx, many, items, longest, full, s.cluster)
+                          : attn_cluster<64, 1, __half>(ctx, many, items, longest, full, s.cluster)
+                   : bf16 ? attn_cluster<64, 2, __nv_bfloat16>(ctx, many, items, longest, full, s.cluster)
+                          : attn_cluster<64, 2, __half>(ctx, many, items, longest, full, s.cluster);
   if (rc) return rc;
   if (s.cluster) {
     s.ctas = static_cast<int>(items * s.cluster);
     return 0;
   }
-  s.chunk = cols >= 64;
+  s.chunk = many;
   if (s.chunk) return 0;
   const int64_t blocks = items * longest;
   s.ctas = static_cast<int>(blocks < full ? blocks : full);
