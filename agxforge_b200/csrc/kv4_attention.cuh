@@ -89,7 +89,7 @@ __device__ __forceinline__ void kv4_write8(const Kv4AttnParams& p, int b, int j,
   *reinterpret_cast<uint4*>(dst) = pack8<T>(v);
 }
 
-// The attention of at least 128 columns a KV head (kv4_chunk.cu).
+// The attention of many columns a KV head (kv4_chunk.cu).
 int launch_kv4_chunk(const agxc_ctx* ctx, const Kv4AttnParams& p, int hd, bool bf16, cudaStream_t s);
 
 }  // namespace agxc

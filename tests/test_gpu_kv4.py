@@ -303,6 +303,9 @@ def test_attention(torch, lens, n, H, KVH, hd, page, dtype, kind):
     ([512], 512, 16, 8, 64, 16, "fp16", "normal"),                   # a prompt from its first token
     ([70, 3, 71, 200, 64, 128, 1, 90] * 3, 70, 8, 8, 128, 32, "fp16", "normal"),
     ([300, 90], 65, 40, 1, 64, 16, "bf16", "normal"),                # forty heads on one KV head
+    ([1, 6, 0, 16] * 20, 10, 32, 8, 128, 16, "fp16", "normal"),      # many sequences of a block at most
+    ([1, 6, 0, 16] * 20, 5, 32, 8, 128, 16, "bf16", "normal"),
+    ([2, 30, 0, 17] * 20, 1, 32, 8, 64, 16, "fp16", "normal"),
     ([900, 40], 77, 32, 8, 128, 64, "fp16", "peaks"),
     ([900, 140], 150, 14, 2, 64, 64, "bf16", "peaks"),
     ([600, 40], 64, 32, 8, 128, 64, "fp16", "spread"),
