@@ -125,6 +125,34 @@ __device__ __forceinline__ bool mbar_wait_quiet(uint64_t* bar, unsigned parity, 
   }
 }
 
+// The bounded waits of a whole warp, which calls them converged: one answer for all 32 lanes. Each lane polls and reads the
+// timer for itself, so around the limit one may give up where its neighbour still sees the phase complete; lanes that went
+// different ways would then meet at the next warp-wide vote, shuffle or MMA, and some of them never. Hence votes.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, unsigned parity, unsigned* err,
+                                               uint64_t limit_ns = 2000000000ull) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (unsigned it = 0;; ++it) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((it & 63u) == 63u && __any_sync(0xffffffffu, globaltimer_ns() - t0 > limit_ns)) {
+      if (err) atomicOr(err, kErrMbarTimeout);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait_quiet_warp(uint64_t* bar, unsigned parity, unsigned* err,
+                                                     uint64_t limit_ns = 2000000000ull) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 200000u))) return true;
+    if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > limit_ns)) {
+      if (err) atomicOr(err, kErrMbarTimeout);
+      return false;
+    }
+  }
+}
+
 // One bulk (non-tensor TMA) copy global -> this CTA's shared memory, completing on `bar` with complete_tx bytes.
 // src and dst 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, unsigned bytes, uint64_t* bar) {

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(p.c.pages);
         if (mine && !ok) atomicOr(p.err, kErrBadPos);
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
-        if (uses >= S && !mbar_wait_quiet(&empty[stage], uses / S - 1 & 1, p.err)) {
+        if (uses >= S && !mbar_wait_quiet_warp(&empty[stage], uses / S - 1 & 1, p.err)) {
           dead = true;
           break;
         }
@@ -266,13 +266,13 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
       }
     }
     // every copy lands before the CTA's memory is another's
-    for (unsigned x = uses < S ? 0 : uses - S; x < uses; ++x) mbar_wait_quiet(&full[x % S], x / S & 1, p.err);
+    for (unsigned x = uses < S ? 0 : uses - S; x < uses; ++x) mbar_wait_quiet_warp(&full[x % S], x / S & 1, p.err);
     if constexpr (!CL) return;
     at.rem = 0;
   }
   const int cl_item = at.item, cl_b = at.b;
 
-  bool dead = false;                        // a wait gave up: the error word says so, and nothing more is computed
+  bool dead = false;                        // a wait of the warp gave up: the error word says so, nothing more is computed
   int slot = 0, phase = 0;
   while (at.rem > 0) {
     const int j = at.item / p.CB, col0 = at.item % p.CB * NC, cols = min(NC, p.n * p.G - col0);
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
     const int end = seen(at);
     bool fresh = true;                       // no key yet: m is set, up or down, by the first ones
     for (int blk = at.t; blk < end; ++blk) {
-      if (!dead && !mbar_wait_bounded(&full[slot], phase, p.err)) dead = true;
+      if (!dead && !mbar_wait_warp(&full[slot], phase, p.err)) dead = true;
       if (dead) continue;
       const unsigned mask = came[slot] >> (2 * warp) & 3u;
       const uint8_t* st = sm + slot * Sm::kStage + warp * 2 * Tile::kBytes;

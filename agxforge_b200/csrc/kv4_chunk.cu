@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
                  &br.raw_full[st]);
     }
     // every copy lands before the memory is used otherwise
-    for (int x = max(0, issued - kRaw); x < issued; ++x) mbar_wait_quiet(&br.raw_full[x % kRaw], x / kRaw & 1, p.err);
+    for (int x = max(0, issued - kRaw); x < issued; ++x) mbar_wait_quiet_warp(&br.raw_full[x % kRaw], x / kRaw & 1, p.err);
   } else if (warp == kMma) {
     // ---- MMAs: the values of block i, then the scores of block i + 2 over the same buffer
     const uint64_t qd = desc_sw128(smem_u32(sm + Sm::kQ)), kd = desc_sw128(smem_u32(sk)), vd = desc_sw128(smem_u32(sv));
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
     // whatever was begun ends before tensor memory is given back
     if (leader) tc_commit(&br.drained);
     __syncwarp();
-    mbar_wait_quiet(&br.drained, 0, p.err);
+    mbar_wait_quiet_warp(&br.drained, 0, p.err);
     }
   } else if (warp >= kDeq) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewerRegs));
