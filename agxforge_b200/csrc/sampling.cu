@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.lo[x] = sh.hi[x] = 0;
   pdl_wait();  // what came before is done from here on
   pdl_launch_dependents();
+  const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;  // of a copy
   if (tid == 0) {
-    const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;
     for (int c = 0; c < kCopies; ++c) {
       const int at = min(bulk, c * each), len = min(bulk, at + each) - at;
       mbar_arrive_expect_tx(&sh.copied[c], len * kSize);
@@ -299,39 +299,51 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                                                 : static_cast<T16>(v == 0.f ? 0u : kMinusInf<DT>);
   };
   float best = -INFINITY, least = INFINITY;
-  int seen = 0;  // copies that have landed
-  for (int q = tid; q < quads; q += kThreads) {
-    const int each = ((bulk + kCopies - 1) / kCopies + 15) / 16 * 16;
-    while (seen < kCopies && seen * each < 4 * q + 4 - pad - head) mbar_wait_bounded(&sh.copied[seen++], 0, p.err);
-    float f[4];
-    get4(q, f);
-    best = fmaxf(fmaxf(best, fmaxf(f[0], f[1])), fmaxf(f[2], f[3]));
-    least = fminf(fminf(least, fminf(f[0], f[1])), fminf(f[2], f[3]));
-    if (f[0] != f[0] || f[1] != f[1] || f[2] != f[2] || f[3] != f[3]) {
+  bool came = true;
+  for (int c = 0, q = tid; c < kCopies; ++c) {  // what each copy brings, as it lands
+    came = came && mbar_wait_warp(&sh.copied[c], 0, p.err);
+    const int end = c + 1 < kCopies ? min(quads, (pad + head + min(bulk, (c + 1) * each)) / 4) : quads;
+    for (; q < end; q += kThreads) {
+      float f[4];
+      get4(q, f);
+      best = fmaxf(fmaxf(best, fmaxf(f[0], f[1])), fmaxf(f[2], f[3]));
+      least = fminf(fminf(least, fminf(f[0], f[1])), fminf(f[2], f[3]));
+      if (f[0] != f[0] || f[1] != f[1] || f[2] != f[2] || f[3] != f[3]) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        if (f[y] != f[y]) {
-          put(4 * q + y, -INFINITY);
-          if (4 * q + y >= pad && 4 * q + y < pad + n) least = -INFINITY;
-        }
+        for (int y = 0; y < 4; ++y)
+          if (f[y] != f[y]) {
+            put(4 * q + y, -INFINITY);
+            if (4 * q + y >= pad && 4 * q + y < pad + n) least = -INFINITY;
+          }
+      }
     }
   }
-  while (seen < kCopies) mbar_wait_bounded(&sh.copied[seen++], 0, p.err);
   best = warp_max(best);
   least = -warp_max(-least);
   if (lane == 0) reinterpret_cast<float2*>(sh.warp64)[warp] = make_float2(best, least);
-  __syncthreads();
+  const bool lost = __syncthreads_or(!came);
   if (warp == 0) {
     const float2 o = lane < kWarps ? reinterpret_cast<float2*>(sh.warp64)[lane] : make_float2(-INFINITY, INFINITY);
     best = warp_max(o.x);
     least = -warp_max(-o.y);
-    if (lane == 0) sh.best = make_float2(best, least);
+    if (lane == 0) sh.best = make_float2(best, lost ? NAN : least);  // NaN: a copy did not land while it was waited for
   }
   cluster.sync();
+  bool whole;
   {
     const float2 o = lane < C ? *cluster.map_shared_rank(&sh.best, lane) : make_float2(-INFINITY, INFINITY);
+    whole = __all_sync(0xffffffffu, o.y == o.y);
     best = warp_max(o.x);
     least = -warp_max(-o.y);
+  }
+  if (!whole) {  // no token from part of a row; the error word says why
+    for (int c = 0; c < kCopies; ++c) mbar_wait_warp(&sh.copied[c], 0, p.err);  // for the copies still on their way
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      p.token[b] = -1;
+      if (p.prob) p.prob[b] = 0.f;
+    }
+    return;
   }
   if (best == -INFINITY || T == 0.f) {  // nothing finite, or greedy: the first maximum
     const bool none = best == -INFINITY || !(1.f >= min_p);

@@ -10,7 +10,7 @@ import pytest
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "agxforge_b200", "csrc")
 # waits on the way out, after which nothing reads what they waited for
 LAST = [r"mbar_wait_quiet_warp\(&full\[x % S\]", r"mbar_wait_quiet_warp\(&br\.raw_full\[x % kRaw\]",
-        r"mbar_wait_quiet_warp\(&br\.drained"]
+        r"mbar_wait_quiet_warp\(&br\.drained", r"mbar_wait_warp\(&sh\.copied\[c\]"]
 
 
 def _source(name):
@@ -29,7 +29,7 @@ def _inside(text, at, opener):
     return False
 
 
-@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_chunk.cu"])
+@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_chunk.cu", "sampling.cu"])
 def test_every_wait_is_the_warps(name):
     text = _source(name)
     waits = list(re.finditer(r"\bmbar_wait_(bounded|quiet)\(", text))
@@ -37,7 +37,7 @@ def test_every_wait_is_the_warps(name):
     assert waits or "mbar_wait_warp(" in text
 
 
-@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_chunk.cu"])
+@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_chunk.cu", "sampling.cu"])
 def test_no_answer_is_dropped(name):
     text = _source(name)
     for m in re.finditer(r"\bmbar_wait_\w+\(", text):
@@ -56,3 +56,12 @@ def test_a_warps_wait_votes():
             assert _inside(body, m.start(), "__all_sync")
         ways = re.findall(r"if \((.*)\) (?:return true;|\{)", body)
         assert len(ways) == 3 and all("__all_sync" in w or "__any_sync" in w for w in ways)
+
+
+def test_a_row_that_did_not_come_gives_no_token():
+    """Sampling: a copy that did not land in time makes the row's token -1, after a second wait for it."""
+    text = _source("sampling.cu")
+    assert "came = came && mbar_wait_warp(" in text and "__syncthreads_or(!came)" in text
+    lost = text[text.index("if (!whole) {"):]
+    lost = lost[:lost.index("return;")]
+    assert "mbar_wait_warp(&sh.copied[c]" in lost and "p.token[b] = -1;" in lost
