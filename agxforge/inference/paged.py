@@ -14,6 +14,8 @@ the GEMVs eight at a time; the append, the attention and the sampler take all of
 """
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import torch
 
@@ -22,6 +24,15 @@ from agxforge.kernels import kv4, sampling
 from agxforge.kernels import qmv as Q
 
 CHUNK = 256          # prompt rows a pass
+
+
+def _on_device(method):
+    """The model's device is current while a method runs: the GEMV calls take the current device's stream."""
+    @functools.wraps(method)
+    def run(self, *args, **kwargs):
+        with torch.cuda.device(self.device):
+            return method(self, *args, **kwargs)
+    return run
 
 
 def _device(a, device):
@@ -39,8 +50,13 @@ class PagedModel:
         self.shape = S = cfg["shape"]
         if S.HEAD_DIM not in (64, 128) or S.HEADS % S.KV_HEADS:
             raise ValueError("PagedModel: head_dim 64 or 128 and heads a multiple of kv_heads")
-        bits, sdt = cfg["bits"], cfg["scale_dtype"]
         self.device, self.page_size = device, page_size
+        with torch.cuda.device(device):
+            self._load(cfg, weights, pages)
+
+    def _load(self, cfg, weights, pages):
+        S, device, page_size = self.shape, self.device, self.page_size
+        bits, sdt = cfg["bits"], cfg["scale_dtype"]
         dev = lambda key: _device(weights[key], device).to(torch.float16)  # noqa: E731
         pack = lambda l, role, n, k: Q.Pack(*weights[(l, role)], n, k, bits, sdt, device)  # noqa: E731
         self.layers = []
@@ -67,6 +83,7 @@ class PagedModel:
         self.cos, self.sin = (_device(f(ang).astype(np.float32), self.device) for f in (np.cos, np.sin))
 
     # ---------------------------------------------------------------- sequences
+    @_on_device
     def add(self, prompt):
         """A sequence with its prompt (at least one token); returns its id. MemoryError where the pages do not reach."""
         toks = [int(t) for t in prompt]
@@ -131,6 +148,7 @@ class PagedModel:
             self.seqs[s]["held"] += n
         return x
 
+    @_on_device
     def logits(self, ids=None):
         """Run the last token of each sequence (all of them by default, in the order of their ids): logits fp32
         [sequences, vocab] of the next one, and the ids."""
@@ -143,6 +161,7 @@ class PagedModel:
         x = self._rows(ids, 1)
         return self._gemv(self.head, x, norm_gain=self.final_gain, eps=self.shape.EPS), ids
 
+    @_on_device
     def step(self, u, ids=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """One token for each sequence, chosen at the uniform numbers u (one a sequence, in the order of the ids); the
         options are sampling.sample's. Returns {id: (token, probability)}."""

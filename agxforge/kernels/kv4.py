@@ -17,9 +17,10 @@ where the fp16 cache takes 16.
                                     0 .. length - rows + i, and a row that sees none gives zeros
     KV4Cache.rows(slots) -> (k, v)  the fp16 values held at some slots
 
-Everything is enqueued on torch's current stream. Shapes and types are checked on the host (ValueError); positions,
-slots, lengths and page numbers live on the device and are checked there: one out of range is left out (a length:
-clamped) and sets a bit of the context's error word, which `check_errors()` reads and raises.
+Everything is enqueued on torch's current stream of the cache's device, whichever device is current. Shapes and types are
+checked on the host (ValueError); positions, slots, lengths and page numbers live on the device and are checked there: one
+out of range is left out (a length: clamped) and sets a bit of the context's error word, which `check_errors()` reads and
+raises.
 """
 from __future__ import annotations
 

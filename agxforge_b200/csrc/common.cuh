@@ -33,6 +33,30 @@ int cuda_fail(cudaError_t e, const char* what);
     if (_e != cudaSuccess) return ::agxc::cuda_fail(_e, #call); \
   } while (0)
 
+// Makes a context's device current for the length of a call and the caller's again at its end: a launch, an attribute and
+// the legacy stream's handle all mean the current device, whatever memory the arguments point to.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    cudaError_t e = cudaGetDevice(&before_);
+    if (e == cudaSuccess && before_ != device) {
+      e = cudaSetDevice(device);
+      moved_ = e == cudaSuccess;
+    }
+    if (e != cudaSuccess) rc_ = cuda_fail(e, "cudaSetDevice");
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  int rc() const { return rc_; }
+
+ private:
+  int before_ = 0, rc_ = 0;
+  bool moved_ = false;
+};
+
 // ----------------------------------------------------------------------------------------------- device helpers
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

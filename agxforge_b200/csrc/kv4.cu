@@ -260,6 +260,8 @@ AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* a, v
   if (reinterpret_cast<uintptr_t>(a->q_dev) % 8) return fail(AGXC_EINVAL, "kv4_append: q must be 8-byte aligned");
   if (static_cast<int64_t>(a->tokens) * (a->heads + 2 * a->cache.kv_heads) > 0x7fffffff)
     return fail(AGXC_EINVAL, "kv4_append: too many tokens for one call");
+  const OnDevice on(ctx->device);
+  if (on.rc()) return on.rc();
   AppendParams p;
   p.c = kv4_of(a->cache);
   p.qkv = a->qkv_dev; p.ld = a->qkv_ld; p.dtype = a->qkv_dtype; p.T = a->tokens; p.H = a->heads;
@@ -289,6 +291,8 @@ AGXC_API int agxc_kv4_rows_dev(agxc_ctx* ctx, const agxc_kv4_cache* cache, const
     return fail(AGXC_EINVAL, "kv4_rows: k and v must be 8-byte aligned");
   const int64_t n = static_cast<int64_t>(tokens) * cache->kv_heads * cache->head_dim / 2;
   if (n > 0x7fffffff - 256) return fail(AGXC_EINVAL, "kv4_rows: too many tokens for one call");
+  const OnDevice on(ctx->device);
+  if (on.rc()) return on.rc();
   const dim3 g(static_cast<unsigned>((n + 255) / 256));
   __half* k = reinterpret_cast<__half*>(k_dev);
   __half* v = reinterpret_cast<__half*>(v_dev);

@@ -894,6 +894,8 @@ AGXC_API int64_t agxc_kv4_attention_workspace(agxc_ctx* ctx, const agxc_kv4_atte
   if (!ctx) return fail(AGXC_EINVAL, "kv4_attention: null context");
   if (attn_check(a)) return -1;
   if (a->batch == 0 || a->rows == 0) return 0;
+  const OnDevice on(ctx->device);
+  if (on.rc()) return -1;
   Shape sh;
   if (attn_shape(ctx, a, sh)) return -1;
   return sh.bytes(a->cache.head_dim);
@@ -907,6 +909,8 @@ AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args
     return fail(AGXC_EINVAL, "kv4_attention: null buffer");
   if (reinterpret_cast<uintptr_t>(a->q_dev) % 16 || reinterpret_cast<uintptr_t>(a->out_dev) % 16)
     return fail(AGXC_EINVAL, "kv4_attention: q and out must be 16-byte aligned");
+  const OnDevice on(ctx->device);
+  if (on.rc()) return on.rc();
   Shape sh;
   if (int rc = attn_shape(ctx, a, sh)) return rc;
   const int64_t need = sh.bytes(a->cache.head_dim);

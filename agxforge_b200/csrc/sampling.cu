@@ -936,6 +936,8 @@ extern "C" AGXC_API int agxc_sample_dev(agxc_ctx* ctx, const agxc_sample_args* a
   if (!a->temperature_dev && !(a->temperature >= 0.f)) return fail(AGXC_EINVAL, "sample: temperature >= 0");
   if (a->batch == 0) return 0;
   if (!a->logits_dev || !a->u_dev || !a->token_dev) return fail(AGXC_EINVAL, "sample: null buffer");
+  const OnDevice on(ctx->device);
+  if (on.rc()) return on.rc();
   SampleParams p;
   p.x = a->logits_dev; p.ld = a->logits_ld; p.B = a->batch; p.V = a->vocab; p.u = a->u_dev;
   p.T = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;

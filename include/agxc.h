@@ -180,7 +180,8 @@ AGXC_API int agxc_argmax_dev(agxc_ctx* ctx, const float* x_dev, int n, int32_t* 
  *     K: t * 32 G + (i / 8) * 8 G + 8 g + i % 8
  *     V: 8 head_dim + (t / 8) * 256 G + (4 (i / 4) + t % 8 / 2) * 8 G + (t % 2) * 4 G + 4 g + i % 4
  * (the order in which the attention's lanes read their tensor-core fragments, 16 bytes at a time).
- * A slot is page * page_size + offset. */
+ * A slot is page * page_size + offset. The calls below run on their context's device, whichever device is current, and
+ * leave the caller's current. */
 #define AGXC_F32 0
 #define AGXC_F16 1
 #define AGXC_BF16 2
