@@ -14,6 +14,7 @@ the GEMVs eight at a time; the append, the attention and the sampler take all of
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 
 import numpy as np
@@ -148,28 +149,45 @@ class PagedModel:
             self.seqs[s]["held"] += n
         return x
 
+    @contextlib.contextmanager
+    def _or_as_before(self, ids):
+        """What fails leaves the sequences as they were: asked for again, the pass writes the same K and V once more."""
+        held = {s: self.seqs[s]["held"] for s in ids}
+        try:
+            yield
+        except BaseException:
+            for s, n in held.items():
+                self.seqs[s]["held"] = n
+            raise
+
+    def _ids(self, ids):
+        return sorted(self.seqs) if ids is None else list(ids)
+
     @_on_device
     def logits(self, ids=None):
         """Run the last token of each sequence (all of them by default, in the order of their ids): logits fp32
         [sequences, vocab] of the next one, and the ids."""
-        ids = sorted(self.seqs) if ids is None else list(ids)
+        ids = self._ids(ids)
         if not ids:
             raise ValueError("logits: no sequence")
         for s in ids:
             if self.seqs[s]["held"] != len(self.seqs[s]["tokens"]) - 1:
                 raise ValueError("logits: sequence %d has no new token" % s)
-        x = self._rows(ids, 1)
-        return self._gemv(self.head, x, norm_gain=self.final_gain, eps=self.shape.EPS), ids
+        with self._or_as_before(ids):
+            x = self._rows(ids, 1)
+            return self._gemv(self.head, x, norm_gain=self.final_gain, eps=self.shape.EPS), ids
 
     @_on_device
     def step(self, u, ids=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """One token for each sequence, chosen at the uniform numbers u (one a sequence, in the order of the ids); the
-        options are sampling.sample's. Returns {id: (token, probability)}."""
-        lg, ids = self.logits(ids)
-        ut = torch.as_tensor(np.asarray(u, np.float32)).to(lg.device).reshape(-1)
-        tok, prob = sampling.sample(lg, ut, temperature, top_k, top_p, min_p)
-        out = {}
-        for s, t, p in zip(ids, tok.tolist(), prob.tolist()):
+        options are sampling.sample's. Returns {id: (token, probability)}; a step that raises leaves the sequences as
+        they were."""
+        ids = self._ids(ids)
+        with self._or_as_before(ids):
+            lg, ids = self.logits(ids)
+            ut = torch.as_tensor(np.asarray(u, np.float32)).to(lg.device).reshape(-1)
+            tok, prob = sampling.sample(lg, ut, temperature, top_k, top_p, min_p)
+            out = dict(zip(ids, zip(tok.tolist(), prob.tolist())))
+        for s, (t, _) in out.items():
             self.seqs[s]["tokens"].append(t)
-            out[s] = (t, p)
         return out
