@@ -188,6 +188,10 @@ class PagedModel:
             ut = torch.as_tensor(np.asarray(u, np.float32)).to(lg.device).reshape(-1)
             tok, prob = sampling.sample(lg, ut, temperature, top_k, top_p, min_p)
             out = dict(zip(ids, zip(tok.tolist(), prob.tolist())))
+            none = [s for s, (t, _) in out.items() if t < 0]
+            if none:
+                raise RuntimeError("step: no token for sequence %s (no finite logit, or a min_p above 1)"
+                                   % ", ".join(map(str, none)))
         for s, (t, _) in out.items():
             self.seqs[s]["tokens"].append(t)
         return out

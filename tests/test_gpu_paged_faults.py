@@ -35,3 +35,19 @@ def test_refused_options_lose_nothing(twins):
             a.step(**bad)
     for _ in range(3):
         assert a.step(u, top_k=20) == b.step(u, top_k=20)
+
+
+def test_no_token(twins):
+    """A row that keeps nothing (min_p above 1) and rows of NaN logits raise; no sequence goes on from token -1."""
+    a, b = twins
+    u = [0.3, 0.6]
+    with pytest.raises(RuntimeError, match="no token"):
+        a.step(u, min_p=2.0)
+    gain = a.final_gain.clone()
+    a.final_gain.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="no token"):
+        a.step(u)
+    a.final_gain.copy_(gain)
+    for _ in range(3):
+        got = a.step(u, temperature=0.8)
+        assert got == b.step(u, temperature=0.8) and min(t for t, _ in got.values()) >= 0

@@ -57,3 +57,14 @@ def test_a_refused_step_can_be_asked_for_again(model):
     assert model.step([0.5, 0.5]) == {0: (7, 0.5), 1: (8, 0.5)}
     assert model.passes[-1] == model.passes[-2]           # the same rows at the same places
     assert state(model) == {0: (3, [1, 2, 3, 7]), 1: (1, [4, 8])}
+
+
+def test_a_row_without_a_token_is_no_token(model):
+    """Token -1 (no finite logit, or a min_p above 1) is no index of the embedding."""
+    before = state(model)
+    model.tokens = [7, -1]
+    with pytest.raises(RuntimeError, match=r"no token for sequence 1\b"):
+        model.step([0.5, 0.5], min_p=2.0)
+    assert state(model) == before
+    model.tokens = [7, 8]
+    assert model.step([0.5, 0.5])[1] == (8, 0.5)
