@@ -214,10 +214,13 @@ def attention(q, cache, page_table, lengths, out=None):
 
 
 def check_errors(device=0):
-    """Wait for the device, read and clear the context's error word, and raise RuntimeError if a call since the last
-    check met a position, slot, length or page out of range."""
+    """Wait for the device, read and clear the error word of its context (the operators of a context share it), and raise if
+    anything set it since the last check: TimeoutError where a bounded wait gave up, RuntimeError otherwise (a position,
+    slot, length or page out of range)."""
     torch.cuda.synchronize(device)
     w = C.c_uint32()
     N.check(N.lib().agxc_ctx_error_word(N.context(device), C.byref(w)), "error_word")
     if w.value:
-        raise RuntimeError("kv4: a position, slot, length or page was out of range (error word 0x%x)" % w.value)
+        what = [text for bit, text in N.ERRORS.items() if w.value & bit] or ["an error"]
+        raise (TimeoutError if w.value & N.ERR_WAITS else RuntimeError)(
+            "kv4: %s (error word 0x%x)" % ("; ".join(what), w.value))

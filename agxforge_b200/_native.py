@@ -17,6 +17,10 @@ OK, EINVAL, ECUDA, ENCCL, ETIMEOUT, ECORRUPT, ENOMEM, EUNSUPPORTED = 0, -1, -2, 
 SCALE_FP16, SCALE_BF16 = 0, 1
 F32, F16, BF16 = 0, 1, 2
 TOKEN_UNSET = 0xFFFFFFFF
+# the bits of a context's error word (csrc/common.cuh); the waits among them raise TimeoutError
+ERRORS = {1: "a bounded device wait gave up", 2: "a token was outside the vocabulary",
+          4: "a position, slot, length or page was out of range", 8: "a grid barrier gave up", 16: "a step was left part-way"}
+ERR_WAITS = 1 | 8
 EPI_F32, EPI_RES1, EPI_RES2, EPI_SWIGLU = 0, 1, 2, 3
 ROLE_QKV, ROLE_WO, ROLE_GATE, ROLE_UP, ROLE_DOWN, ROLE_HEAD = range(6)
 VEC_ATTN_GAIN, VEC_FFN_GAIN, VEC_QKV_BIAS, VEC_FINAL_GAIN, VEC_EMBED, VEC_Q_NORM, VEC_K_NORM = range(7)
