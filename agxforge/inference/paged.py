@@ -86,7 +86,8 @@ class PagedModel:
     # ---------------------------------------------------------------- sequences
     @_on_device
     def add(self, prompt):
-        """A sequence with its prompt (at least one token); returns its id. MemoryError where the pages do not reach."""
+        """A sequence with its prompt (at least one token); returns its id. MemoryError where the pages do not reach; what
+        raises leaves no sequence behind."""
         toks = [int(t) for t in prompt]
         if not toks or min(toks) < 0 or max(toks) >= self.shape.VOCAB:
             raise ValueError("add: a prompt of at least one token of the vocabulary")
@@ -96,7 +97,8 @@ class PagedModel:
             while self.seqs[s]["held"] < len(toks) - 1:
                 n = min(CHUNK, len(toks) - 1 - self.seqs[s]["held"])
                 self._rows([s], n)
-        except MemoryError:
+            kv4.check_errors(self.device)
+        except BaseException:
             self.free(s)
             raise
         return s
@@ -161,21 +163,26 @@ class PagedModel:
             raise
 
     def _ids(self, ids):
-        return sorted(self.seqs) if ids is None else list(ids)
+        ids = sorted(self.seqs) if ids is None else list(ids)
+        if not ids:
+            raise ValueError("logits: no sequence")
+        for s in ids:
+            if self.seqs[s]["held"] != len(self.seqs[s]["tokens"]) - 1:
+                raise ValueError("logits: sequence %d has no new token" % s)
+        return ids
+
+    def _logits(self, ids):
+        return self._gemv(self.head, self._rows(ids, 1), norm_gain=self.final_gain, eps=self.shape.EPS)
 
     @_on_device
     def logits(self, ids=None):
         """Run the last token of each sequence (all of them by default, in the order of their ids): logits fp32
         [sequences, vocab] of the next one, and the ids."""
         ids = self._ids(ids)
-        if not ids:
-            raise ValueError("logits: no sequence")
-        for s in ids:
-            if self.seqs[s]["held"] != len(self.seqs[s]["tokens"]) - 1:
-                raise ValueError("logits: sequence %d has no new token" % s)
         with self._or_as_before(ids):
-            x = self._rows(ids, 1)
-            return self._gemv(self.head, x, norm_gain=self.final_gain, eps=self.shape.EPS), ids
+            lg = self._logits(ids)
+            kv4.check_errors(self.device)
+        return lg, ids
 
     @_on_device
     def step(self, u, ids=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -184,10 +191,11 @@ class PagedModel:
         they were."""
         ids = self._ids(ids)
         with self._or_as_before(ids):
-            lg, ids = self.logits(ids)
+            lg = self._logits(ids)
             ut = torch.as_tensor(np.asarray(u, np.float32)).to(lg.device).reshape(-1)
             tok, prob = sampling.sample(lg, ut, temperature, top_k, top_p, min_p)
             out = dict(zip(ids, zip(tok.tolist(), prob.tolist())))
+            kv4.check_errors(self.device)
             none = [s for s, (t, _) in out.items() if t < 0]
             if none:
                 raise RuntimeError("step: no token for sequence %s (no finite logit, or a min_p above 1)"

@@ -51,3 +51,16 @@ def test_no_token(twins):
     for _ in range(3):
         got = a.step(u, temperature=0.8)
         assert got == b.step(u, temperature=0.8) and min(t for t, _ in got.values()) >= 0
+
+
+def test_the_error_word_is_read(twins):
+    """A page outside the cache in a sequence's table: its keys would be missing without a word."""
+    a, b = twins
+    pages = a.seqs[0]["pages"]
+    good = pages[0]
+    for call in (lambda: a.step([0.3, 0.6]), a.logits):
+        pages[0] = 1000
+        with pytest.raises(RuntimeError, match="out of range"):
+            call()
+        pages[0] = good
+    assert a.step([0.3, 0.6]) == b.step([0.3, 0.6])

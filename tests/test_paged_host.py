@@ -68,3 +68,27 @@ def test_a_row_without_a_token_is_no_token(model):
     assert state(model) == before
     model.tokens = [7, 8]
     assert model.step([0.5, 0.5])[1] == (8, 0.5)
+
+
+def test_a_pass_that_went_wrong_on_the_device_raises(model, monkeypatch):
+    """A wait that gave up, a page out of range: nothing is returned, nothing counts as held."""
+    before = state(model)
+    model.tokens = [7, 8]
+    bad = []
+
+    def check(device=0):
+        if bad:
+            raise TimeoutError(bad.pop())
+
+    monkeypatch.setattr(kv4, "check_errors", check)
+    for call in (lambda: model.step([0.5, 0.5]), lambda: model.logits()):
+        bad.append("a bounded device wait gave up")
+        with pytest.raises(TimeoutError, match="gave up"):
+            call()
+        assert state(model) == before and not bad
+    spare = list(model.spare)
+    bad.append("a bounded device wait gave up")
+    with pytest.raises(TimeoutError):
+        model.add([5, 6, 7])
+    assert state(model) == before and model.spare == spare
+    assert model.step([0.5, 0.5]) == {0: (7, 0.5), 1: (8, 0.5)}
