@@ -166,6 +166,8 @@ class PagedModel:
         ids = sorted(self.seqs) if ids is None else list(ids)
         if not ids:
             raise ValueError("logits: no sequence")
+        if len(set(ids)) != len(ids):
+            raise ValueError("logits: a sequence named twice")
         for s in ids:
             if self.seqs[s]["held"] != len(self.seqs[s]["tokens"]) - 1:
                 raise ValueError("logits: sequence %d has no new token" % s)

@@ -92,3 +92,14 @@ def test_a_pass_that_went_wrong_on_the_device_raises(model, monkeypatch):
         model.add([5, 6, 7])
     assert state(model) == before and model.spare == spare
     assert model.step([0.5, 0.5]) == {0: (7, 0.5), 1: (8, 0.5)}
+
+
+def test_a_sequence_named_twice_is_refused(model):
+    """Its one new token would be two rows at two places, the second past its end."""
+    before = state(model)
+    model.tokens = [7, 8]
+    for call in (lambda: model.logits([0, 0]), lambda: model.step([0.5, 0.5, 0.5], [1, 0, 1])):
+        with pytest.raises(ValueError, match="twice"):
+            call()
+    assert state(model) == before
+    assert model.step([0.5, 0.5], [1, 0]) == {1: (7, 0.5), 0: (8, 0.5)}
