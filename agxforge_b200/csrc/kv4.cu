@@ -4,7 +4,9 @@
 //            o2 = x2 c + x1 s, each product and sum rounded (as the fp16 cache's append); q = o * qscale, rounded;
 //            k and v quantised per 64 dims: scale = (max - min) fp32(1 / 15) and bias = min in fp16 (scale 1 where all are
 //            equal), code = rint((x - b) / s) clipped to 0..15, 0 where that is not finite; each step an IEEE fp32
-//            operation, so the codes do not depend on how the tokens are batched.
+//            operation, so the codes do not depend on how the tokens are batched. A NaN makes its group's bias NaN and with
+//            it the whole group: the minimum and maximum keep it, where fminf and fmaxf would drop it and store a broken
+//            value as the group's least.
 //   rows     scale * code + bias of given slots, one fused multiply-add, rounded to fp16.
 #include "kv4.cuh"
 
@@ -57,13 +59,25 @@ __device__ __forceinline__ void load4(const void* p, int64_t i, bool vec, float*
   }
 }
 
+// the smaller and the larger of two, NaN where either is
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // min and max over the LPH lanes of a head
 template <int LPH>
 __device__ __forceinline__ void head_minmax(float& lo, float& hi) {
 #pragma unroll
   for (int m = LPH / 2; m >= 1; m >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
   }
 }
 
@@ -133,12 +147,12 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   float lo[2], hi[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    lo[h] = fminf(fminf(x[4 * h], x[4 * h + 1]), fminf(x[4 * h + 2], x[4 * h + 3]));
-    hi[h] = fmaxf(fmaxf(x[4 * h], x[4 * h + 1]), fmaxf(x[4 * h + 2], x[4 * h + 3]));
+    lo[h] = min_nan(min_nan(x[4 * h], x[4 * h + 1]), min_nan(x[4 * h + 2], x[4 * h + 3]));
+    hi[h] = max_nan(max_nan(x[4 * h], x[4 * h + 1]), max_nan(x[4 * h + 2], x[4 * h + 3]));
   }
   if (HD == 64) {
-    lo[0] = lo[1] = fminf(lo[0], lo[1]);
-    hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
+    lo[0] = lo[1] = min_nan(lo[0], lo[1]);
+    hi[0] = hi[1] = max_nan(hi[0], hi[1]);
   }
   head_minmax<LPH>(lo[0], hi[0]);
   if (HD == 128) head_minmax<LPH>(lo[1], hi[1]);

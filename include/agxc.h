@@ -213,8 +213,8 @@ typedef struct {
 } agxc_kv4_append_args;
 
 /* Rotates each token's q and k (fp32, two rounded products and one rounded sum an output), scales and rounds q, and
- * writes k and v into the cache in 4 bits. A position outside the tables or a slot past the cache sets the error word
- * (kErrBadPos) and leaves that token out. tokens = 0 does nothing. */
+ * writes k and v into the cache in 4 bits; a NaN makes its group of 64 dims NaN. A position outside the tables or a slot
+ * past the cache sets the error word (kErrBadPos) and leaves that token out. tokens = 0 does nothing. */
 AGXC_API int agxc_kv4_append_dev(agxc_ctx* ctx, const agxc_kv4_append_args* args, void* stream);
 
 /* The values the cache holds at `tokens` slots, fp16 [tokens][kv_heads][head_dim] each, 8-byte aligned (zeros for a
