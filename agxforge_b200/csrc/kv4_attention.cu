@@ -22,8 +22,9 @@
 // share of that line, whatever the lengths are. A fifth warp copies the blocks, a bulk copy a tile (which is
 // contiguous), into three stages of shared memory, and each of four warps computes on 32 keys of a block. A piece that
 // is not a whole item leaves its maximum, sum and values in the workspace, and a second kernel joins the pieces in a
-// fixed order (no atomics: equal calls give equal bits). Few items are split over a cluster each instead, whose CTAs join
-// their pieces in shared memory: one launch, and no second kernel to wait for.
+// fixed order (no atomics: equal calls give equal bits). A sum of weights is zero where no key was seen; one that is NaN,
+// from a query or a seen key that is not finite, is carried along like any other. Few items are split over a cluster each
+// instead, whose CTAs join their pieces in shared memory: one launch, and no second kernel to wait for.
 //
 // 64 sequences of 8,192 tokens, 32 heads over 8 KV heads of 128 dims (605 MB): 133 us, 4.55 TB/s (the copy rate would take
 // 92.5). The SM's issue slots bind it, 59 of 100 taken at 12 warps an SM, with DRAM at 56: two ANDs, a subtraction and their
@@ -168,7 +169,7 @@ __device__ __forceinline__ void join_lanes(int lanes, float m, float sum, float*
 #pragma unroll
   for (int x = 8; x >= 1; x >>= 1)
     if (x < lanes) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-  const float inv = sum > 0.f ? f / sum : 0.f;
+  const float inv = sum != 0.f ? f / sum : 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] *= inv;
 #pragma unroll
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         float sum = l[nt][e];
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        if (r == 0) sml[warp * NC + col] = make_float2(sum > 0.f ? m[nt][e] : kNone, sum);
+        if (r == 0) sml[warp * NC + col] = make_float2(sum != 0.f ? m[nt][e] : kNone, sum);
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
           float bias = bt[nt][g][e];
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         for (int e = 0; e < 8; ++e) v[e] = fmaf(f, src[e], v[e]);
       }
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
         kv4_write8<HD, T>(p, at.b, j, col0 + col, d, v);
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
       const int u = min(u0 + (lane >> lg), units - 1), col = u / (HD / 8), d = u % (HD / 8) * 8, x = lane & (p.cluster - 1);
       float v[8] = {};
       const float2 ml = *cluster.map_shared_rank(reinterpret_cast<float2*>(sm + Sm::kOwn) + col, x);
-      if (ml.y > 0.f) {
+      if (ml.y != 0.f) {
         const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(so + col * Sm::kRow + d, x));
         const float4 a = src[0], e = src[1];
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(64 * NT, 16 / NT) kv4_join_kernel(const __grid
 #pragma unroll 4
         for (long long x = c0; x <= c1; ++x) t.add(ml, val, (2 * x + (x == c0)) * NC + col, d);
       }
-      const float inv = t.sum > 0.f ? 1.f / t.sum : 0.f;
+      const float inv = t.sum != 0.f ? 1.f / t.sum : 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) t.v[e] *= inv;
       kv4_write8<HD, T>(p, b, j, col0 + col, d, t.v);

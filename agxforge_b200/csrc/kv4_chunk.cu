@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
     float* out = reinterpret_cast<float*>(sk) + row * Sm::kRow;
     float2* ml = reinterpret_cast<float2*>(sm + Sm::kMl) + row;
     if (grp == 0) {
-      *ml = make_float2(l > 0.f ? m : kNone, l);
+      *ml = make_float2(l != 0.f ? m : kNone, l);
       if (done)
 #pragma unroll
         for (int x = 0; x < HD / 32; ++x) {
@@ -611,11 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
     asm volatile("bar.sync 3, 256;" ::: "memory");
     if (grp == 1) {
       const float2 other = *ml;
-      const float mm = fmaxf(l > 0.f ? m : kNone, other.x);
-      float f1 = l > 0.f ? ex2(m - mm) : 0.f, f0 = other.y > 0.f ? ex2(other.x - mm) : 0.f;
+      const float mm = fmaxf(l != 0.f ? m : kNone, other.x);  // a sum that is NaN goes along
+      float f1 = l != 0.f ? ex2(m - mm) : 0.f, f0 = other.y != 0.f ? ex2(other.x - mm) : 0.f;
       const float sum = f1 * l + f0 * other.y;
       if (cp.S == 1) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
         f0 *= inv;
         f1 *= inv;
       } else {
@@ -632,8 +632,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
         for (int e = 0; e < 32; e += 8) {
           float v[8];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) v[y] = f1 > 0.f ? fmaf(o[e + y], y & 1 ? c : a, z) : 0.f;
-          if (f0 > 0.f) {
+          for (int y = 0; y < 8; ++y) v[y] = f1 != 0.f ? fmaf(o[e + y], y & 1 ? c : a, z) : 0.f;
+          if (f0 != 0.f) {
 #pragma unroll
             for (int y = 0; y < 8; y += 4) {
               const float4 u = *reinterpret_cast<const float4*>(out + 32 * x + e + y);
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
       }
 #pragma unroll
       for (int x = 0; x < kMaxShare; ++x)
-        if (ml[x].y > 0.f) {
+        if (ml[x].y != 0.f) {
           const float f = ex2(ml[x].x - mx);
           const float4* src = reinterpret_cast<const float4*>(
               cluster.map_shared_rank(reinterpret_cast<float*>(sk) + r * Sm::kRow + d, x));
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
           v[0] = fmaf(f, a.x, v[0]); v[1] = fmaf(f, a.y, v[1]); v[2] = fmaf(f, a.z, v[2]); v[3] = fmaf(f, a.w, v[3]);
           v[4] = fmaf(f, e.x, v[4]); v[5] = fmaf(f, e.y, v[5]); v[6] = fmaf(f, e.z, v[6]); v[7] = fmaf(f, e.w, v[7]);
         }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= inv;
       kv4_write8<HD, T>(p, b, j, col0 + r, d, v);

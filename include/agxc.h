@@ -236,8 +236,9 @@ typedef struct {
 } agxc_kv4_attention_args;
 
 /* Attention over the 4-bit cache for `rows` query rows of each sequence: row i sees keys 0 .. length - rows + i (a row
- * that sees none gives zeros); q head h reads KV head h / (heads / kv_heads). A length outside 0 .. max_pages *
- * page_size is clamped and a page outside the cache is read as no keys; both set the error word (kErrBadPos). */
+ * that sees none gives zeros); q head h reads KV head h / (heads / kv_heads). A row whose query or seen keys hold a NaN
+ * gives NaN. A length outside 0 .. max_pages * page_size is clamped and a page outside the cache is read as no keys; both
+ * set the error word (kErrBadPos). */
 AGXC_API int64_t agxc_kv4_attention_workspace(agxc_ctx* ctx, const agxc_kv4_attention_args* args);
 AGXC_API int agxc_kv4_attention_dev(agxc_ctx* ctx, const agxc_kv4_attention_args* args, void* stream);
 
