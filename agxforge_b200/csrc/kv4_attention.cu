@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         }
       }
       if (key0 + 32 > least || mask != 3u) {  // the mask's edge: an unseen key weighs nothing, whatever its bytes hold
+        bool odd = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -434,7 +435,27 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
 #pragma unroll
               for (int g = 0; g < GR; ++g) ve[h][i][g] = 0u;
             }
+#pragma unroll
+            for (int g = 0; g < GR; ++g) odd |= !finite_pair(ve[h][i][g]);
           }
+        // A V that is not finite, of a key that only some of the rows see: it counts here, for the columns that see it,
+        // because a weight of zero times it would not be zero for the others.
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int g = 0; g < GR; ++g) {
+                if (finite_pair(ve[h][i][g])) continue;
+                ve[h][i][g] = 0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (key0 + h * 16 + r + 8 * i < lim[nt][e]) bt[nt][g][e] = NAN;
+              }
+        }
       }
       // Has a weight or a scale outgrown its reference? The weights' sums of this lane's keys tell of the first (over
       // 4,096 where one passes 2^12), each lane looks at the scales of one key for the second.
@@ -469,7 +490,8 @@ __global__ void __launch_bounds__(kThreads + 32, NT == 1 ? 3 : 2)
         float fg[GR];
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
-          const float up = fmaxf(sref[g], __uint_as_float((__float_as_uint(warp_max(big[g])) + 0x7fffffu) & 0x7f800000u));
+          const uint32_t top = __float_as_uint(warp_max(finite_abs(big[g])));
+          const float up = fmaxf(sref[g], __uint_as_float((top + 0x7fffffu) & 0x7f800000u));
           fg[g] = sref[g] / up;
           sref[g] = up;
           isref[g] = 1.f / up;

@@ -39,6 +39,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// the size of an fp16 scale, 0 where it is not finite: the running power of two above the scales is every row's
+__device__ __forceinline__ float finite_abs(float s) { return fabsf(s) <= 65504.f ? fabsf(s) : 0.f; }
+
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -46,6 +49,12 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ float2 bits_float2(uint32_t u) { return __half22float2(as_half2(u)); }
+
+// are an entry's scale and bias finite?
+__device__ __forceinline__ bool finite_pair(uint32_t u) {
+  const float2 v = bits_float2(u);
+  return fabsf(v.x) + fabsf(v.y) <= 131008.f;
+}
 
 __device__ __forceinline__ void unpack8(const uint4& u, float* f, const __half*) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};

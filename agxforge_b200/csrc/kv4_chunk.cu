@@ -44,6 +44,7 @@ constexpr int kMoreRegs = 160, kFewerRegs = 96;
 constexpr int kRaw = 3, kSt = 3;                                // raw stages, operand stages
 constexpr int kTmemCols = 512, kD = 256;
 constexpr float kNone = -1e30f;
+constexpr unsigned kOdd = 16u;                                  // some V of the block is not finite
 constexpr int kMaxShare = 8;                                    // CTAs an item: what a portable cluster has
 
 template <int HD>
@@ -68,7 +69,8 @@ struct Bars {
   uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[kSt], kv_done[kSt], s_full[2], p_full[2], pv_done[2], drained;
   uint32_t tmem;
   volatile int dead;
-  volatile unsigned came_raw[kRaw], came[kSt];
+  volatile unsigned came_raw[kRaw], came[kSt];   // bits 0 .. 3: the tiles that were copied; kOdd
+  volatile unsigned odd[kSt][2][2];              // [group][half of the keys] whose V is not finite, where kOdd is set
   volatile float sref[kSt][2];
 };
 
@@ -360,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
       }
       if (w == 0) {  // the table; a key that did not come counts as one of no weight (its scores are masked)
         float f[2][8] = {}, big[GR] = {};
+        unsigned bad = 0u;  // V's entries that are not finite: bit 2 g + z
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const int key = z * 32 + lane;
@@ -369,9 +372,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
           for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
             for (int g = 0; g < GR; ++g) {
-              const float2 sb = __half22float2(e[kv * GR + g]);
-              f[z][4 * kv + g] = in ? sb.x : 0.f;
-              f[z][4 * kv + 2 + g] = in ? fmaf(8.f, sb.x, sb.y) : 0.f;
+              const uint32_t u = *reinterpret_cast<const uint32_t*>(e + kv * GR + g);
+              const bool fine = kv == 0 || finite_pair(u);
+              const float2 sb = bits_float2(u);
+              if (in && !fine) bad |= 1u << (2 * g + z);
+              f[z][4 * kv + g] = in && fine ? sb.x : 0.f;
+              f[z][4 * kv + 2 + g] = in && fine ? fmaf(8.f, sb.x, sb.y) : 0.f;
             }
 #pragma unroll
           for (int g = 0; g < GR; ++g) big[g] = fmaxf(big[g], fabsf(f[z][4 + g]));
@@ -393,8 +399,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
             to[8] = f[z][4 + g] / sref[g];
             to[12] = f[z][6 + g];
           }
+        // They go into the sums of the columns that see them, not into the table: a weight of zero times one of them would
+        // not be zero for the columns that do not.
+        const bool odd = __any_sync(0xffffffffu, bad != 0u);
+        if (odd) {
+#pragma unroll
+          for (int x = 0; x < 2 * GR; ++x) {
+            const unsigned keys = __ballot_sync(0xffffffffu, bad >> x & 1u);
+            if (lane == 0) br.odd[st][x >> 1][x & 1] = keys;
+          }
+        }
         if (lane == 0) {
-          br.came[st] = mask;
+          br.came[st] = odd ? mask | kOdd : mask;
           br.sref[st][0] = sref[0];
           br.sref[st][1] = sref[GR - 1];
         }
@@ -473,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
         break;
       tc_fence_after();
       const ulonglong2* table = reinterpret_cast<const ulonglong2*>(sm + Sm::kTable) + st * kKeys * 2;
-      const unsigned mask = br.came[st];
+      const unsigned came = br.came[st], mask = came & 0xFu;
       const int key0 = (first + i) * kKeys;
       float y[kKeys], mx = -INFINITY;
       const f2 minus_m = pair(-m, -m);
@@ -504,6 +520,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_con
 #pragma unroll
         for (int k = 0; k < kKeys; ++k)
           if (key0 + k >= lim || !(mask >> (k >> 4) & 1u)) y[k] = -INFINITY;
+      }
+      if (came & kOdd) {
+        const int keys = lim - key0;  // that the column sees
+#pragma unroll
+        for (int g = 0; g < GR; ++g)
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            if (keys > 32 * z && (br.odd[st][g][z] & (keys >= 32 * z + 32 ? 0xffffffffu : (1u << (keys - 32 * z)) - 1u)))
+              bt2[g] = pair(NAN, NAN);
       }
 #pragma unroll
       for (int k = 0; k < kKeys; ++k) mx = fmaxf(mx, y[k]);

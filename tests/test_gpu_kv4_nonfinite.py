@@ -67,7 +67,8 @@ def _entry(torch, cache, table, b, t, which):
 
 
 @pytest.mark.parametrize("lens,n,H,KVH,hd,page,dtype", FEW + LINE + MANY)
-@pytest.mark.parametrize("which,part,bad", [(0, 0, "nan"), (0, 1, "nan")])
+@pytest.mark.parametrize("which,part,bad", [(0, 0, "nan"), (0, 1, "nan"), (1, 0, "nan"), (1, 1, "nan"), (1, 0, "inf"),
+                                            (1, 1, "-inf")])
 def test_attention_keys(torch, lens, n, H, KVH, hd, page, dtype, which, part, bad):
     """One scale or bias of K (which = 0) or V of some keys is not finite, in one KV head and one group of dims."""
     from agxforge.kernels import kv4
