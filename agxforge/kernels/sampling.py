@@ -8,7 +8,9 @@ logits by index (NaN ranks as -inf); weights are exp((l - max) / T) in whole uni
 gives the same token whatever batch it is in. Kept are the first `top_k` ranks (top_k <= 0: all), of those the ranks
 whose weight before them is below top_p of the total (top_p >= 1: all; the first always), of those the weights >=
 min_p (of the largest). The token is the first kept index at which the cumulative weight exceeds u of the total, and
-prob its share of the kept weight. Temperature 0 takes the first maximum; a row with no finite logit gives -1 and 0.
+prob its share of the kept weight. Temperature 0 takes the first maximum; a row with no finite logit, or that keeps nothing
+(min_p above 1), gives -1 and 0. So does a temperature of an array that is below 0 or NaN, and it sets a bit of the error
+word that kv4.check_errors reads; a number like that is refused (ValueError).
 """
 from __future__ import annotations
 

@@ -19,7 +19,8 @@ F32, F16, BF16 = 0, 1, 2
 TOKEN_UNSET = 0xFFFFFFFF
 # the bits of a context's error word (csrc/common.cuh); the waits among them raise TimeoutError
 ERRORS = {1: "a bounded device wait gave up", 2: "a token was outside the vocabulary",
-          4: "a position, slot, length or page was out of range", 8: "a grid barrier gave up", 16: "a step was left part-way"}
+          4: "a position, slot, length or page was out of range", 8: "a grid barrier gave up", 16: "a step was left part-way",
+          32: "a sampling option was out of range"}
 ERR_WAITS = 1 | 8
 EPI_F32, EPI_RES1, EPI_RES2, EPI_SWIGLU = 0, 1, 2, 3
 ROLE_QKV, ROLE_WO, ROLE_GATE, ROLE_UP, ROLE_DOWN, ROLE_HEAD = range(6)

@@ -21,6 +21,7 @@ constexpr unsigned kErrBadToken = 1u << 1;
 constexpr unsigned kErrBadPos = 1u << 2;
 constexpr unsigned kErrGridTimeout = 1u << 3;  // a grid barrier of the persistent step gave up
 constexpr unsigned kErrAbort = 1u << 4;        // a wait gave up: every other wait of the launch leaves too
+constexpr unsigned kErrBadOption = 1u << 5;    // a sampling option out of range
 
 // ----------------------------------------------------------------------------------------------- host errors
 void set_error(const std::string& msg);

@@ -266,8 +266,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (tail < nc) cache[pad + tail] = src[tail];
     else if (nc == n && pad + tail < 4 * quads) cache[pad + tail] = static_cast<T16>(kNaN<DT>);
   }
-  const float T = fminf(p.T_a ? p.T_a[b] : p.T, FLT_MAX), top_p = p.p_a ? p.p_a[b] : p.top_p,
-              min_p = p.m_a ? p.m_a[b] : p.min_p;
+  const float T_in = p.T_a ? p.T_a[b] : p.T, top_p = p.p_a ? p.p_a[b] : p.top_p, min_p = p.m_a ? p.m_a[b] : p.min_p;
+  const bool no_T = !(T_in >= 0.f);  // below zero, where weights would pass 1 and leave the sums' range, or NaN
+  const float T = fminf(T_in, FLT_MAX);
   const int k_in = p.k_a ? p.k_a[b] : p.top_k;
   const bool use_k = k_in > 0 && k_in < p.V, use_p = top_p < 1.f;
   __syncthreads();
@@ -345,8 +346,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  if (best == -INFINITY || T == 0.f) {  // nothing finite, or greedy: the first maximum
-    const bool none = best == -INFINITY || !(1.f >= min_p);
+  if (best == -INFINITY || T == 0.f || no_T) {  // nothing finite or no temperature: none; greedy: the first maximum
+    const bool none = best == -INFINITY || no_T || !(1.f >= min_p);
+    if (no_T && rank == 0 && tid == 0) atomicOr(p.err, kErrBadOption);
     if (!none) {
       int first = 0x7fffffff;
       for (int q = tid; q < quads && first == 0x7fffffff; q += kThreads) {

@@ -262,7 +262,8 @@ typedef struct {
  * in whole units of 2^-40, so every sum is exact and no result depends on an order of addition. Kept: the first top_k
  * ranks (top_k <= 0: all); of those the ranks whose weight before them is below ceil(top_p * total) (top_p >= 1: all,
  * and always the first); of those the weights >= min_p. The token is the first kept index whose cumulative weight
- * exceeds floor(u * total), and prob its weight / total. T = 0: the first maximum, prob 1. No finite logit: -1, 0. */
+ * exceeds floor(u * total), and prob its weight / total. T = 0: the first maximum, prob 1. No finite logit: -1, 0. A
+ * temperature of the array that is below zero or NaN: -1, 0 and the error word (kErrBadOption). */
 AGXC_API int agxc_sample_dev(agxc_ctx* ctx, const agxc_sample_args* args, void* stream);
 
 /* ---- the model (agxforge/inference/assemble.py configure 71-92, build 596-828; models.py 26-54) -------------- */
