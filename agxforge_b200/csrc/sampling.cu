@@ -268,7 +268,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   const float T_in = p.T_a ? p.T_a[b] : p.T, top_p = p.p_a ? p.p_a[b] : p.top_p, min_p = p.m_a ? p.m_a[b] : p.min_p;
   const bool no_T = !(T_in >= 0.f);  // below zero, where weights would pass 1 and leave the sums' range, or NaN
-  const float T = fminf(T_in, FLT_MAX);
+  // from the smallest normal number up, so that 1 / T is finite (only logits that are subnormal numbers themselves could
+  // tell: any other below the maximum is further away than 28 T)
+  const float T = T_in > 0.f ? fminf(fmaxf(T_in, FLT_MIN), FLT_MAX) : T_in;
   const int k_in = p.k_a ? p.k_a[b] : p.top_k;
   const bool use_k = k_in > 0 && k_in < p.V, use_p = top_p < 1.f;
   __syncthreads();

@@ -1,4 +1,5 @@
-"""Options at the ends of their ranges, on the B200: values that are no temperature."""
+"""Options at the ends of their ranges, on the B200: temperatures below fp32's normal numbers, values that are no
+temperature."""
 import numpy as np
 import pytest
 
@@ -13,6 +14,23 @@ def torch():
     if not t.cuda.is_available():
         pytest.skip("no GPU")
     return t
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T", [1e-30, 1e-37, 1.1754944e-38, 1e-38, 3e-39, 1e-40, 1.4e-45])
+def test_the_smallest_temperatures(torch, T, dtype):
+    """All the weight on the maximum: at these temperatures any other logit is further below than 2^-40 reaches."""
+    from agxforge.kernels import sampling
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(_logits(rng, 5, 5003)).to(getattr(torch, dtype)).cuda()
+    x[torch.arange(5), torch.tensor([0, 17, 4000, 5002, 333])] = 40.0
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24], device="cuda")
+    array = torch.full((5,), T, device="cuda")
+    assert bool((array > 0).all())
+    for t in (T, array):
+        for k, p, least in [(0, 1.0, 0.0), (50, 1.0, 0.0), (0, 0.9, 0.0), (7, 0.9, 0.05)]:
+            token, prob = sampling.sample(x, u, t, k, p, least)
+            assert token.tolist() == [0, 17, 4000, 5002, 333] and prob.tolist() == [1.0] * 5, (k, p, least)
 
 
 def test_values_that_are_no_temperature(torch):
