@@ -48,6 +48,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     m, md = _option(min_p, torch.float32, B, idx, "min_p")
     if not t >= 0:
         raise ValueError("sample: temperature >= 0")
+    if not -1 <= k <= V:           # all of them; the call takes 32 bits
+        k = 0
     dev = logits.device
     tokens = torch.empty(B, dtype=torch.int32, device=dev)
     probs = torch.empty(B, dtype=torch.float32, device=dev)

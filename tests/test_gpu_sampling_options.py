@@ -1,5 +1,5 @@
-"""Options at the ends of their ranges, on the B200: temperatures below fp32's normal numbers, values that are no
-temperature."""
+"""Options at the ends of their ranges, on the B200: temperatures below fp32's normal numbers, values that are no temperature,
+and a top_k past 32 bits."""
 import numpy as np
 import pytest
 
@@ -59,3 +59,14 @@ def test_values_that_are_no_temperature(torch):
     for t in (-1.0, float("nan"), -1e-40):
         with pytest.raises(ValueError, match="temperature"):
             sampling.sample(x, u, t)
+
+
+def test_top_k_past_32_bits(torch):
+    from agxforge.kernels import sampling
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(_logits(rng, 3, 1000)).cuda()
+    u = torch.tensor([0.1, 0.5, 0.9], device="cuda")
+    want = sampling.sample(x, u, 2.0)
+    for k in (1000, (1 << 31) - 1, 1 << 31, (1 << 32) + 1, 1 << 40, -(1 << 31) - 1, -(1 << 32) + 1):
+        got = sampling.sample(x, u, 2.0, k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
