@@ -198,12 +198,14 @@ def attention(q, cache, page_table, lengths, out=None):
     a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), kind, B, n, H, page_table.data_ptr(),
                            page_table.stride(0) if B > 1 else mp, mp, lengths.data_ptr(), None, 0)
     L, ctx = N.lib(), N.context(idx)
-    need = cache._workspace.get((B, n, H, mp))
+    need = cache._workspace.get((kind, B, n, H, mp))
     if need is None:
         need = L.agxc_kv4_attention_workspace(ctx, C.byref(a))
         if need < 0:
             N.check(N.EINVAL, "attention")
-        cache._workspace[B, n, H, mp] = need
+        if len(cache._workspace) >= 1024:
+            cache._workspace.clear()
+        cache._workspace[kind, B, n, H, mp] = need
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
         a.workspace_dev, a.workspace_bytes = ws.data_ptr(), need
