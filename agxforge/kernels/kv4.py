@@ -195,8 +195,11 @@ def attention(q, cache, page_table, lengths, out=None):
         _check(out, q.dtype, idx, "attention: out")
         _need(out.shape == shape, "attention: out has q's shape")
     mp = pages[1]
-    a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), kind, B, n, H, page_table.data_ptr(),
-                           page_table.stride(0) if B > 1 else mp, mp, lengths.data_ptr(), None, 0)
+    ld = page_table.stride(0) if B > 1 else mp
+    if ld > 0x7fffffff:
+        raise ValueError("attention: page_table rows less than 2^31 entries apart")
+    a = N.Kv4AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), kind, B, n, H, page_table.data_ptr(), ld, mp,
+                           lengths.data_ptr(), None, 0)
     L, ctx = N.lib(), N.context(idx)
     need = cache._workspace.get((kind, B, n, H, mp))
     if need is None:

@@ -37,3 +37,15 @@ def test_the_workspace_is_asked_for_per_type(torch, monkeypatch):
         c._workspace[("shape", rows)] = 0
     kv4.attention(torch.zeros((1, 3, 4, 64), dtype=torch.float16, device="cuda"), c, table, lens)
     assert len(c._workspace) <= 1024
+
+
+def test_a_page_tables_stride_past_32_bits(torch):
+    """Rows further apart than the call can say are refused, not taken from elsewhere."""
+    from agxforge.kernels import kv4
+    c = kv4.KV4Cache(2, 2, 64, 16)
+    store = torch.zeros((1 << 32) + 8, dtype=torch.int32, device="cuda")
+    q, lens = torch.zeros((2, 4, 64), dtype=torch.float16, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    for stride in (1 << 31, (1 << 32) + 2):
+        with pytest.raises(ValueError, match="page_table"):
+            kv4.attention(q, c, store.as_strided((2, 2), (stride, 1)), lens)
+    kv4.attention(q, c, store.as_strided((2, 2), (1000, 1)), lens)
