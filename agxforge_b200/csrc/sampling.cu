@@ -28,6 +28,7 @@
 // the top-p rows, 43 for the 33), a pass of their own for the kept weights (310).
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cfloat>
 
 #include "common.cuh"
@@ -877,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 // (64 rows of 92,544: 24.2 us with four CTAs a row, one an SM; 26.6 with eight, two an SM in two waves).
 template <int DT>
 int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
-  static int most[64] = {};  // the largest cluster that the device places
+  static std::atomic<int> most[64] = {};  // the largest cluster that the device places
   int dev = 0;
   AGXC_CUDA(cudaGetDevice(&dev));
   if (dev >= 64) return fail(AGXC_EINVAL, "sample: device index below 64");

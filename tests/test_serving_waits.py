@@ -65,3 +65,10 @@ def test_a_row_that_did_not_come_gives_no_token():
     lost = text[text.index("if (!whole) {"):]
     lost = lost[:lost.index("return;")]
     assert "mbar_wait_warp(&sh.copied[c]" in lost and "p.token[b] = -1;" in lost
+
+
+@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_chunk.cu", "sampling.cu"])
+def test_what_launches_remember_is_atomic(name):
+    """Calls of different threads meet in the tables of what a device takes (the binding lets go of the interpreter's lock)."""
+    kept = re.findall(r"\bstatic (?!constexpr|const |_)([\w:<> ]+?) (\w+)\[", _source(name))
+    assert kept and all(kind.startswith("std::atomic<") for kind, _ in kept), kept
