@@ -89,8 +89,9 @@ __device__ __forceinline__ unsigned code4(float x, float s, float b) {
 // hd / 8 lanes a head: lane l holds dims 4l .. 4l + 3 and the dims hd / 2 above them (four RoPE pairs, two code bytes
 // side by side each). A warp takes two heads of 128 or four of 64.
 // Every value is read once and each lane's loads, codes and q are one access each; 3,585 tokens of 14 + 2 x 2 heads of 64
-// with the read back of their rows: 11.6 us (single values a lane took 14.0), where the bytes alone, 18.6 MB, take 2.8: what
-// is left are two launches and one wave of short chains, load, exchange over the head's lanes, divide, store. One token: 3.9.
+// with the read back of their rows: 11.3 us (single values a lane took 14.0), where the bytes alone, 18.6 MB, take 2.8. The
+// append's 2,017 CTAs of 40 registers are 2.3 waves of six an SM, and the issue slots are 65 of 100 taken: chains of load,
+// exchange over the head's lanes, divide, store, the exchange run for the q heads too, which do not use it. One token: 3.5.
 template <int HD, int DT>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
   using Tile = Kv4Tile<HD>;

@@ -26,11 +26,11 @@
 // from a query or a seen key that is not finite, is carried along like any other. Few items are split over a cluster each
 // instead, whose CTAs join their pieces in shared memory: one launch, and no second kernel to wait for.
 //
-// 64 sequences of 8,192 tokens, 32 heads over 8 KV heads of 128 dims (605 MB): 133 us, 4.55 TB/s (the copy rate would take
-// 92.5). The SM's issue slots bind it, 59 of 100 taken at 12 warps an SM, with DRAM at 56: two ANDs, a subtraction and their
+// 64 sequences of 8,192 tokens, 32 heads over 8 KV heads of 128 dims (605 MB): 135 us, 4.48 TB/s (the copy rate would take
+// 92.5). The SM's issue slots bind it, 59 of 100 taken at 12 warps an SM, with DRAM at 53: two ANDs, a subtraction and their
 // share of an MMA for each pair of codes of K and V, about 300 instructions a 16-key tile and warp where 475 took 197 us.
-// 128 ragged sequences of up to 1,792 tokens of 2 KV heads of 64 (18.6 MB): 18 us; one of 1,792 of 8: 6.7, both a launch, a
-// chain of three dependent loads and a join. 16 rows of 8 sequences: 23 us, the 32 columns a KV head as two blocks, which
+// 128 ragged sequences of up to 1,792 tokens of 2 KV heads of 64 (18.6 MB): 18.6 us; one of 1,792 of 8: 6.7, both a launch, a
+// chain of three dependent loads and a join. 16 rows of 8 sequences: 22 us, the 32 columns a KV head as two blocks, which
 // dequantise each key twice. Not kept: compute warps that take the copy's turn (156 us), seven of them in two CTAs an
 // SM (136), codes or-ed into 1,024 (148).
 #include <cooperative_groups.h>

@@ -17,9 +17,9 @@
 // Tensor memory: two O, two D (and P): 512 columns, one CTA an SM. Few items: a cluster of CTAs shares the keys of one
 // item and joins through distributed shared memory.
 //
-// 256 rows of 32 heads over 8 KV heads, 2,304 keys of 128 dims (9.1 GFLOP, 5.5 us at the measured peak): 41.7 us; the
+// 256 rows of 32 heads over 8 KV heads, 2,304 keys of 128 dims (9.1 GFLOP, 5.5 us at the measured peak): 41.4 us; the
 // kernel of single tokens, whose mma.sync dequantises each key once per 16 columns, takes 81.5. 512 rows over 8,192 keys:
-// 216 us, 1.7 us a block of 64 keys and 128 columns, 0.97 at 64 dims. What bounds it is the shared memory pipe, busy for 80
+// 218 us, 1.7 us a block of 64 keys and 128 columns, 0.97 at 64 dims. What bounds it is the shared memory pipe, busy for 80
 // of 100 cycles on the SMs that work: each softmax warp reads every key's scales and biases (1,020 of a block's 2,060
 // wavefronts; a read of 16 bytes by all lanes costs two), the dequantised operands are written (390) and the tensor core reads
 // them (500). Tried and not kept: P through shared memory instead of tensor memory (49 us), scores fetched 16 keys at a

@@ -18,14 +18,14 @@
 //      than a list (thousands of equal logits) is cut bit by bit
 //   5  the kept weights' total and the token, in index order: the warp, then the element, that the target falls on
 //
-// 256 rows of 151,936 fp32 logits (155.6 MB, 23.8 us at the copy rate), eight CTAs a row, 37 rows at a time: 55 us greedy,
-// 122 with the weights alone, 145 with top-k 50, 283 with top-p 0.95, 187 where rows mix all of these. The SMs bind it, not
-// DRAM (fetching the next rows into L2 meanwhile gained nothing): of a top-p row's time 5 us go to loading it and its
-// maximum, 9.6 to the weights in bins (an exp and a shared-memory add each), 3.6 to the first CTA's sum of the cluster's
-// bins, 6 to the list of the cut's bin and the weights above it, 2.7 to the cut and 2 to the draw, and the cluster's
-// barriers between them leave warps waiting. One row with top-k 50: 13.8 us, steps and barriers; 64 rows of 92,544 with
-// min-p: 24.2; 33 rows of 50,257 bf16, top-k 1,000: 28. Not kept: the listed keys sorted in place of finer bins (382 for
-// the top-p rows, 43 for the 33), a pass of their own for the kept weights (310).
+// 256 rows of 151,936 fp32 logits (155.6 MB, 23.8 us at the copy rate), eight CTAs a row, 37 rows at a time: 52 us greedy,
+// 118 with the weights alone, 144 with top-k 50, 278 with top-p 0.95, 184 where rows mix all of these. The SMs bind it, not
+// DRAM (fetching the next rows into L2 meanwhile gained nothing): of a top-p row's time (by clock, when the rows took 283) 5 us
+// went to loading it and its maximum, 9.6 to the weights in bins (an exp and a shared-memory add each), 3.6 to the first CTA's
+// sum of the cluster's bins, 6 to the list of the cut's bin and the weights above it, 2.7 to the cut and 2 to the draw, and
+// the cluster's barriers between them leave warps waiting. One row with top-k 50: 12.9 us, steps and barriers; 64 rows of
+// 92,544 with min-p: 22.3; 33 rows of 50,257 bf16, top-k 1,000: 27.4. Not kept: the listed keys sorted in place of finer bins
+// (382 for the top-p rows, 43 for the 33), a pass of their own for the kept weights (310).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -874,8 +874,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   cluster.sync();  // the neighbours' shared memory stays until all have read it
 }
 
-// CTAs a row: doubled while the rows' CTAs are no more than the SMs, and so many that a CTA's range takes at most 96 KB
-// (64 rows of 92,544: 24.2 us with four CTAs a row, one an SM; 26.6 with eight, two an SM in two waves).
+// CTAs a row: doubled while the rows' CTAs are no more than the SMs, and so many that a CTA's range takes at most 96 KB. That
+// limit was measured at one size, 64 rows of 92,544: 24.2 us with four CTAs a row, of 122,688 bytes each and so one an SM, 26.6
+// with eight, two an SM; either way two waves.
 template <int DT>
 int sample_launch(const agxc_ctx* ctx, SampleParams p, cudaStream_t s) {
   static std::atomic<int> most[64] = {};  // the largest cluster that the device places
